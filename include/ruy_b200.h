@@ -50,7 +50,12 @@ typedef enum ruyb200_dtype {
   RUYB200_I16 = 2,
   RUYB200_I32 = 3,
   RUYB200_F32 = 4,
-  RUYB200_F64 = 5   /* only in ruy's mixed float cases: (f64, f32, f64, f32) and (f32, f64, f64, f64) */
+  RUYB200_F64 = 5,  /* only in ruy's mixed float cases: (f64, f32, f64, f32) and (f32, f64, f64, f64) */
+  /* Not among ruy's scalar types; only ruyb200_mul_q4_async and ruyb200_mul_grouped_q4_async take them. */
+  RUYB200_F16 = 6,
+  RUYB200_BF16 = 7,
+  RUYB200_I4 = 8,   /* two's complement, two to a byte, the element of the lower index in the low half */
+  RUYB200_U4 = 9
 } ruyb200_dtype;
 
 /* ruy::Order (ruy/matrix.h:30). */
@@ -92,7 +97,10 @@ enum {
   RUYB200_KERNEL_SGEMM = 3,     /* fp32 FFMA tiled kernel (small shapes) */
   RUYB200_KERNEL_GEMV = 4,      /* narrow muls (at most 8 destination rows or columns): one pass over the wide operand */
   RUYB200_KERNEL_BATCH_I8 = 5,  /* persistent many-small-muls kernel (plans) */
-  RUYB200_KERNEL_TC_F32 = 6     /* fp32 on tcgen05 kind::tf32: hi/lo split operands, three products, short accumulation chains */
+  RUYB200_KERNEL_TC_F32 = 6,    /* fp32 on tcgen05 kind::tf32: hi/lo split operands, three products, short accumulation chains */
+  RUYB200_KERNEL_GROUPED_TC = 7,   /* grouped 8-bit muls: tcgen05 kind::i8, tiles found on the device from the offsets */
+  RUYB200_KERNEL_GROUPED_MMA = 8,  /* grouped 8-bit muls of few columns per group: one pass over the weights, register-level MMAs */
+  RUYB200_KERNEL_Q4 = 9            /* 4-bit weights: copy-engine staged, widened to bf16 / f16 in registers, register-level MMAs */
 };
 
 /* A non-owning matrix view: ruy::Matrix<T> / ruy::Mat<T> (ruy/matrix.h:132-165,
@@ -233,6 +241,66 @@ RUYB200_API int ruyb200_validate(const ruyb200_mul_desc* desc);
  * (different streams or threads) race on it and must be serialised by the caller.
  * rounding_mode RUYB200_ROUNDING_FROM_PATH means the reference rounding here. */
 RUYB200_API int ruyb200_mul_noalloc(const ruyb200_mul_desc* desc, void* cuda_stream);
+
+/* ---- weights in groups and weights of 4 bits -------------------------------------------------- */
+
+/* Additive: ruy has one LHS per mul and no type below 8 bits.  What follows serves the two forms in which the weight
+ * products of current language models differ from that: several weight matrices of one shape, each multiplied with
+ * its own run of the columns (the experts of a mixture-of-experts layer), and weights of 4 bits with a scale for every
+ * block of the depth.
+ *
+ * All three calls are stream-ordered like ruyb200_mul_async: they validate, enqueue on the context's stream and return
+ * without synchronizing.  Every pointer must be device (or managed) memory of the context's device.  They allocate
+ * nothing and use no scratch memory, so they may be captured into CUDA graphs, any number of which may run at once.
+ * Device-side lists (offsets, zero points) are read when the kernel runs; nothing of them is read on the host.
+ *
+ * ruyb200_groups: column c of rhs and dst belongs to group g when offsets[g] <= c < offsets[g + 1].  The LHS of group g
+ * starts lhs_stride * g elements after lhs.data, its bias and per-channel multipliers channel_stride * g entries after
+ * the first ones (0: all groups share them), its scales and zero points scale_stride * g entries after the first ones.
+ * offsets is int32[count + 1] in device memory and should not decrease.  Columns outside every group are left as they
+ * were; an entry outside [0, cols] counts as the nearer end of that range, and a group that ends before it begins is
+ * empty.  At most 1024 groups. */
+typedef struct ruyb200_groups {
+  const int32_t* offsets;
+  int64_t lhs_stride;
+  int64_t channel_stride;
+  int64_t scale_stride;   /* 4-bit weights only */
+  int32_t count;
+  int32_t reserved;
+} ruyb200_groups;
+
+/* The scales of 4-bit weights: element (r, k) of the LHS stands for scale[r][k / block] * (q - zero_point[r][k / block]).
+ * One row's entries are contiguous, the next row's start `stride` entries later (stride >= ceil(depth / block)); the
+ * zero points, where given, are laid out like the scales and lie within the weights' type ([-8, 7] or [0, 15]). */
+typedef struct ruyb200_q4_scales {
+  const void* scales;
+  const int8_t* zero_points;   /* NULL: all 0 */
+  int32_t block;               /* depth that shares one scale: a multiple of 32 */
+  int32_t stride;
+  uint8_t dtype;               /* RUYB200_F32, RUYB200_F16 or RUYB200_BF16 */
+  uint8_t reserved[7];
+} ruyb200_q4_scales;
+
+/* dst[:, c] = the mul that `desc` describes of group g's LHS with rhs[:, c], for every column c of every group g.
+ * desc->lhs describes group 0's weights (rows x depth), desc->rhs all columns, desc->dst all destination columns.
+ * 8-bit operands, int32 accumulation, destinations int8, uint8, int16 or int32, with ruy's whole integer epilogue; bit-exact
+ * with ruyb200_mul on each group.  Per-channel buffers run along the rows (RUYB200_CHANNEL_ROW) when there are any.  LHS
+ * row-major, RHS and dst column-major; cache policies are ignored, the weights are used where they are.  Base addresses,
+ * strides and lhs_stride that are multiples of 16 bytes (lhs_stride also of the row stride) run on the tensor cores,
+ * anything else on a slower CUDA-core kernel. */
+RUYB200_API int ruyb200_mul_grouped_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, const ruyb200_groups* groups);
+/* dst = clamp(bias + W * rhs) with W of 4 bits, for the few columns of decoding (any number is computed; the cost of
+ * streaming the weights recurs for every 8 to 32 columns).  desc->lhs: RUYB200_I4 or RUYB200_U4, row-major, stride in
+ * elements and even, zero_point 0.  desc->rhs: RUYB200_F32, F16 or BF16, any order and stride.  desc->dst: F32 or the
+ * type of rhs, any order and stride.  desc->params: accum_dtype RUYB200_F32, bias float[rows] or NULL, clamp_* in .f; NaN
+ * results stay NaN whatever the clamp.  Sums are held in 32 bits; they may be formed over (part of) a block before its
+ * scale is applied.  Weights whose base address is a multiple of 16
+ * bytes and whose stride is one of 32 elements (lhs_stride also of the row stride) run on the tensor cores, anything
+ * else on a slower CUDA-core kernel. */
+RUYB200_API int ruyb200_mul_q4_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, const ruyb200_q4_scales* scales);
+/* The same with groups: group g's LHS and scales multiply the columns of group g. */
+RUYB200_API int ruyb200_mul_grouped_q4_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, const ruyb200_q4_scales* scales,
+                                             const ruyb200_groups* groups);
 
 /* ---- plans: many independent muls in one launch ------------------------ */
 

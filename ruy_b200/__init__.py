@@ -6,7 +6,7 @@ This Python package is the host-side mirror of ruy's API used by the tests and
 the benchmark.
 """
 from .api import (  # noqa: F401
-    CachePolicy, ChannelDimension, Context, Layout, Matrix, MulParams, Order, Path,
-    PerformanceAdvisory, Plan, Rounding, RuyError, kAllPaths, kDefaultPaths,
-    make_desc, make_simple_layout, mul, mul_async, mul_noalloc, validate,
+    CachePolicy, ChannelDimension, Context, Groups, Layout, Matrix, MulParams, Order, Path,
+    PerformanceAdvisory, Plan, Q4Matrix, Q4Scales, Rounding, RuyError, kAllPaths, kDefaultPaths,
+    make_desc, make_simple_layout, mul, mul_async, mul_grouped_async, mul_grouped_q4_async, mul_noalloc, mul_q4_async, validate,
 )

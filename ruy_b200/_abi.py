@@ -15,9 +15,10 @@ STATUS_NAMES = {
 }
 
 # ruyb200_dtype
-I8, U8, I16, I32, F32, F64 = 0, 1, 2, 3, 4, 5
-DTYPE_SIZE = {I8: 1, U8: 1, I16: 2, I32: 4, F32: 4, F64: 8}
-NUMPY_DTYPE = {I8: "int8", U8: "uint8", I16: "int16", I32: "int32", F32: "float32", F64: "float64"}
+I8, U8, I16, I32, F32, F64, F16, BF16, I4, U4 = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
+DTYPE_SIZE = {I8: 1, U8: 1, I16: 2, I32: 4, F32: 4, F64: 8, F16: 2, BF16: 2}
+NUMPY_DTYPE = {I8: "int8", U8: "uint8", I16: "int16", I32: "int32", F32: "float32", F64: "float64", F16: "float16",
+               BF16: "bfloat16"}
 DTYPE_OF_NUMPY = {v: k for k, v in NUMPY_DTYPE.items()}
 
 COL_MAJOR, ROW_MAJOR = 0, 1
@@ -29,7 +30,9 @@ PATH_INTERNAL_VARIANT1, PATH_INTERNAL_VARIANT2, PATH_INTERNAL_VARIANT3 = 0x2, 0x
 PATH_AVX, PATH_AVX2_FMA, PATH_AVX512 = 0x10, 0x20, 0x40
 ADVISORY_NONE, ADVISORY_REALLOCATED_PERCHANNEL_BUFFER = 0, 1
 KERNEL_NONE, KERNEL_GENERIC, KERNEL_TC_I8, KERNEL_SGEMM, KERNEL_GEMV, KERNEL_BATCH_I8, KERNEL_TC_F32 = 0, 1, 2, 3, 4, 5, 6
-KERNEL_NAMES = {0: "none", 1: "generic", 2: "tc_i8", 3: "sgemm", 4: "gemv", 5: "batch_i8", 6: "tc_f32"}
+KERNEL_GROUPED_TC, KERNEL_GROUPED_MMA, KERNEL_Q4 = 7, 8, 9
+KERNEL_NAMES = {0: "none", 1: "generic", 2: "tc_i8", 3: "sgemm", 4: "gemv", 5: "batch_i8", 6: "tc_f32", 7: "grouped_tc",
+                8: "grouped_mma", 9: "q4"}
 
 
 class MatrixDesc(C.Structure):
@@ -76,6 +79,30 @@ class MulDesc(C.Structure):
         ("rhs", MatrixDesc),
         ("dst", MatrixDesc),
         ("params", MulParamsDesc),
+    ]
+
+
+class GroupsDesc(C.Structure):
+    """ruyb200_groups."""
+    _fields_ = [
+        ("offsets", C.c_void_p),
+        ("lhs_stride", C.c_int64),
+        ("channel_stride", C.c_int64),
+        ("scale_stride", C.c_int64),
+        ("count", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class Q4ScalesDesc(C.Structure):
+    """ruyb200_q4_scales."""
+    _fields_ = [
+        ("scales", C.c_void_p),
+        ("zero_points", C.c_void_p),
+        ("block", C.c_int32),
+        ("stride", C.c_int32),
+        ("dtype", C.c_uint8),
+        ("reserved", C.c_uint8 * 7),
     ]
 
 
@@ -143,6 +170,9 @@ PROTOTYPES = {
     "ruyb200_cache_export": (C.c_int, [C.c_void_p, _P(MatrixDesc), C.c_int, C.c_void_p, _P(C.c_size_t)]),
     "ruyb200_cache_import": (C.c_int, [C.c_void_p, _P(MatrixDesc), C.c_int, C.c_void_p, C.c_size_t]),
     "ruyb200_mul_noalloc": (C.c_int, [_P(MulDesc), C.c_void_p]),
+    "ruyb200_mul_grouped_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(GroupsDesc)]),
+    "ruyb200_mul_q4_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(Q4ScalesDesc)]),
+    "ruyb200_mul_grouped_q4_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(Q4ScalesDesc), _P(GroupsDesc)]),
     "ruyb200_plan_create": (C.c_int, [C.c_void_p, _P(MulDesc), C.c_int, _P(C.c_void_p)]),
     "ruyb200_plan_run": (C.c_int, [C.c_void_p]),
     "ruyb200_plan_destroy": (C.c_int, [C.c_void_p]),

@@ -91,14 +91,17 @@ def _is_torch(x):
     return type(x).__module__.startswith("torch")
 
 
+_torch_codes = {}   # torch dtype -> ruyb200_dtype, filled when the first tensor comes by
+
+
 def _ptr_and_dtype(data):
     if data is None:
         return None, None
     if _is_torch(data):
-        import torch
-        names = {torch.int8: "int8", torch.uint8: "uint8", torch.int16: "int16",
-                 torch.int32: "int32", torch.float32: "float32", torch.float64: "float64"}
-        return data.data_ptr(), _abi.DTYPE_OF_NUMPY[names[data.dtype]]
+        if not _torch_codes:
+            import torch
+            _torch_codes.update({getattr(torch, name): code for name, code in _abi.DTYPE_OF_NUMPY.items()})
+        return data.data_ptr(), _torch_codes[data.dtype]
     a = data
     return a.ctypes.data, _abi.DTYPE_OF_NUMPY[a.dtype.name]
 
@@ -286,6 +289,78 @@ def mul_noalloc(lhs, rhs, mul_params, dst, stream=None):
     device-resident depth-contiguous operands, at most 16384 x 16384 destinations).  Synchronous."""
     d = make_desc(lhs, rhs, mul_params, dst)
     _check(lib().ruyb200_mul_noalloc(C.byref(d), C.c_void_p(stream) if stream else None), "ruyb200_mul_noalloc")
+
+
+class Groups:
+    """Columns in ragged groups, each with weights of its own (ruyb200_groups): column c of rhs and dst belongs to group g
+    when offsets[g] <= c < offsets[g + 1].  `offsets` is an int32 device tensor of count + 1 entries, read when the kernel
+    runs; the strides are in elements of what they step over."""
+
+    def __init__(self, offsets, lhs_stride, channel_stride=0, scale_stride=0):
+        self.offsets = offsets
+        self.lhs_stride = lhs_stride
+        self.channel_stride = channel_stride
+        self.scale_stride = scale_stride
+
+    def to_desc(self):
+        ptr, dt = _ptr_and_dtype(self.offsets)
+        if dt != _abi.I32:
+            raise TypeError("Groups.offsets must be int32")
+        return _abi.GroupsDesc(ptr, self.lhs_stride, self.channel_stride, self.scale_stride, max(0, len(self.offsets) - 1))
+
+
+class Q4Scales:
+    """Scales of 4-bit weights (ruyb200_q4_scales): one per row and `block` of the depth, `stride` entries from one row's
+    to the next row's; `zero_points`, if any, are int8 and laid out alike."""
+
+    def __init__(self, scales, block, stride, zero_points=None):
+        self.scales = scales
+        self.block = block
+        self.stride = stride
+        self.zero_points = zero_points
+
+    def to_desc(self):
+        ptr, dt = _ptr_and_dtype(self.scales)
+        zp, zdt = _ptr_and_dtype(self.zero_points)
+        if zdt not in (None, _abi.I8):
+            raise TypeError("Q4Scales.zero_points must be int8")
+        return _abi.Q4ScalesDesc(ptr, zp, self.block, self.stride, dt if dt is not None else 0)
+
+
+class Q4Matrix:
+    """A row-major matrix of 4-bit weights: `data` holds two elements to a byte, the one of the lower index in the low
+    half (a uint8 or int8 tensor); `layout` counts elements (its stride is even)."""
+
+    def __init__(self, data, layout, scales, signed=True):
+        self.data = data
+        self.layout = layout
+        self.scales = scales
+        self.signed = signed
+
+    def to_desc(self):
+        lay = self.layout
+        return _abi.MatrixDesc(_ptr_and_dtype(self.data)[0], lay.rows, lay.cols, lay.stride, 0, lay.order,
+                               _abi.I4 if self.signed else _abi.U4, 0, 0)
+
+
+def mul_grouped_async(lhs, rhs, mul_params, context, dst, groups):
+    """ruyb200_mul_grouped_async: the 8-bit mul of every group's weights with that group's columns, in one launch.  `lhs`
+    describes the first group's weights.  Stream-ordered, device-resident operands."""
+    d, g = make_desc(lhs, rhs, mul_params, dst), groups.to_desc()
+    _check(lib().ruyb200_mul_grouped_async(context._h, C.byref(d), C.byref(g)), "ruyb200_mul_grouped_async")
+
+
+def mul_q4_async(lhs, rhs, mul_params, context, dst):
+    """ruyb200_mul_q4_async: 4-bit weights (a Q4Matrix) times a few columns of float, half or bfloat16 activations.
+    Stream-ordered, device-resident operands."""
+    d, q = make_desc(lhs, rhs, mul_params, dst), lhs.scales.to_desc()
+    _check(lib().ruyb200_mul_q4_async(context._h, C.byref(d), C.byref(q)), "ruyb200_mul_q4_async")
+
+
+def mul_grouped_q4_async(lhs, rhs, mul_params, context, dst, groups):
+    """ruyb200_mul_grouped_q4_async: mul_q4_async with groups."""
+    d, q, g = make_desc(lhs, rhs, mul_params, dst), lhs.scales.to_desc(), groups.to_desc()
+    _check(lib().ruyb200_mul_grouped_q4_async(context._h, C.byref(d), C.byref(q), C.byref(g)), "ruyb200_mul_grouped_q4_async")
 
 
 def cache_blob_info(blob):

@@ -38,6 +38,7 @@ int ctx_fail(int status, const char* msg);
 int ctx_validate(const ruyb200_mul_desc* d);
 bool ptr_on_device(const void* p);
 int ctx_rounding_is_x86(ruyb200_ctx* ctx, int rounding_mode);
+bool ctx_trace(ruyb200_ctx* ctx);
 int ctx_run_mul_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* d);
 int ctx_plan_item(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, BatchItem* out, bool* fits,
                   std::vector<CacheKey>* pinned);
