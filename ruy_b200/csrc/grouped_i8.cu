@@ -1,4 +1,10 @@
 // Grouped 8-bit muls (ruyb200_mul_grouped_async).
+#include <cuda.h>
+
+#include <cstring>
+
+#include "async.cuh"
+#include "batch_i8.h"
 #include "grouped.h"
 
 namespace ruyb200 {
@@ -55,12 +61,534 @@ cudaError_t launch_any(const GroupedI8Mul& m, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// ---- few columns per group: register-level MMAs --------------------------------------------------------
+//
+// Bound by the weights' bytes.  A CTA owns 16 weight rows of a group and its warps split the depth; every weight byte is
+// loaded once per 8 or 16 columns, straight into MMA fragments (m16n8k32): the depth may be taken in any order as long as
+// both operands take the same, so a lane's 16 consecutive bytes are its share of two MMAs.  Sums for the zero points come
+// from the same registers.  CTAs of empty groups leave at once.
+constexpr int kMmaWarps = 4;
+
+template <bool kWSigned, bool kXSigned>
+__device__ __forceinline__ void mma_16832(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+#define RUYB200_MMA(A, B)                                                                                             \
+  asm("mma.sync.aligned.m16n8k32.row.col.s32." A "." B ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                                \
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if (kWSigned && kXSigned) RUYB200_MMA("s8", "s8");
+  else if (kWSigned) RUYB200_MMA("s8", "u8");
+  else if (kXSigned) RUYB200_MMA("u8", "s8");
+  else RUYB200_MMA("u8", "u8");
+#undef RUYB200_MMA
+}
+
+template <bool kSigned>
+__device__ __forceinline__ int32_t add4(uint32_t v, int32_t sum) {
+  return kSigned ? __dp4a((int)v, 0x01010101, sum) : (int32_t)__dp4a(v, 0x01010101u, (uint32_t)sum);
+}
+template <bool kSigned>
+__device__ __forceinline__ int32_t add16(const uint4& v, int32_t sum) {
+  return add4<kSigned>(v.w, add4<kSigned>(v.z, add4<kSigned>(v.y, add4<kSigned>(v.x, sum))));
+}
+
+// 16 bytes of a row from position k on; those at and beyond `depth` count as 0 and are not read.
+__device__ __forceinline__ uint4 load_piece(const uint8_t* row, int k, int depth, bool stream) {
+  if (k + 16 <= depth) return stream ? __ldcs(reinterpret_cast<const uint4*>(row + k)) : __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    if (k + i < depth) w[i / 4] |= (uint32_t)__ldg(row + k + i) << (8 * (i % 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool kWSigned, bool kXSigned, int kTiles>
+__global__ void __launch_bounds__(32 * kMmaWarps) grouped_i8_mma_kernel(const __grid_constant__ GroupedI8Mul m) {
+  constexpr int kPart = 5 * kTiles + 2;   // per lane: 4 sums and an activation sum per tile of 8 columns, 2 weight sums
+  __shared__ int32_t part[kMmaWarps - 1][kPart][32];
+  const int g = blockIdx.y;
+  int begin, end;
+  group_columns(m.groups, g, m.cols, &begin, &end);
+  if (begin == end) return;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, quad = lane >> 2, t = lane & 3;
+  const int r0 = blockIdx.x * 16 + quad, r1 = r0 + 8;
+  const uint8_t* const base = (const uint8_t*)m.w + (int64_t)g * m.groups.lhs_stride;
+  const uint8_t* const row0 = base + (int64_t)min(r0, m.rows - 1) * m.w_stride;
+  const uint8_t* const row1 = base + (int64_t)min(r1, m.rows - 1) * m.w_stride;
+  const bool need_w = m.zp_x != 0, need_x = m.zp_w != 0;
+  for (int c0 = begin; c0 < end; c0 += 8 * kTiles) {
+    int32_t acc[kTiles][4] = {}, xsum[kTiles] = {}, wsum0 = 0, wsum1 = 0;
+    const uint8_t* xrow[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; j++) {
+      // columns past the group's last repeat it; their sums are not stored
+      xrow[j] = (const uint8_t*)m.x + (int64_t)min(c0 + 8 * j + quad, end - 1) * m.x_stride;
+    }
+    // a step is 256 bytes of every row: 4 pieces of 16 per lane, all loads before the first use
+    for (int k0 = warp * 256; k0 < m.depth; k0 += 256 * kMmaWarps) {
+      uint4 a[4], b[4], x[kTiles][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        a[i] = load_piece(row0, k0 + 64 * i + 16 * t, m.depth, true);
+        b[i] = load_piece(row1, k0 + 64 * i + 16 * t, m.depth, true);
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[j][i] = load_piece(xrow[j], k0 + 64 * i + 16 * t, m.depth, false);
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          mma_16832<kWSigned, kXSigned>(acc[j], a[i].x, b[i].x, a[i].y, b[i].y, x[j][i].x, x[j][i].y);
+          mma_16832<kWSigned, kXSigned>(acc[j], a[i].z, b[i].z, a[i].w, b[i].w, x[j][i].z, x[j][i].w);
+          if (need_x) xsum[j] = add16<kXSigned>(x[j][i], xsum[j]);
+        }
+      }
+      if (need_w) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          wsum0 = add16<kWSigned>(a[i], wsum0);
+          wsum1 = add16<kWSigned>(b[i], wsum1);
+        }
+      }
+    }
+    if (warp > 0) {
+#pragma unroll
+      for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) part[warp - 1][5 * j + e][lane] = acc[j][e];
+        part[warp - 1][5 * j + 4][lane] = xsum[j];
+      }
+      part[warp - 1][5 * kTiles][lane] = wsum0;
+      part[warp - 1][5 * kTiles + 1][lane] = wsum1;
+    }
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 0; w < kMmaWarps - 1; w++) {
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[j][e] += part[w][5 * j + e][lane];
+          xsum[j] += part[w][5 * j + 4][lane];
+        }
+        wsum0 += part[w][5 * kTiles][lane];
+        wsum1 += part[w][5 * kTiles + 1][lane];
+      }
+      // the lanes of a quad hold the quarters of each step
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {
+        wsum0 += __shfl_xor_sync(0xffffffffu, wsum0, d);
+        wsum1 += __shfl_xor_sync(0xffffffffu, wsum1, d);
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) xsum[j] += __shfl_xor_sync(0xffffffffu, xsum[j], d);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int r = h ? r1 : r0;
+        const bool there = r < m.rows;
+        const int64_t ch = (int64_t)g * m.groups.channel_stride + r;
+        const int32_t bias = there && m.bias ? m.bias[ch] : 0;
+        const int32_t mfp = there && m.mfp_pc ? m.mfp_pc[ch] : m.mfp;
+        const int32_t mexp = there && m.mexp_pc ? m.mexp_pc[ch] : m.mexp;
+        const uint32_t row_term = (uint32_t)bias - (uint32_t)m.zp_x * (uint32_t)(h ? wsum1 : wsum0) +
+                                  (uint32_t)m.zp_x * (uint32_t)m.zp_w * (uint32_t)m.depth;
+#pragma unroll
+        for (int j = 0; j < kTiles; j++) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int c = 8 * j + 2 * t + e;
+            const int32_t xs = __shfl_sync(0xffffffffu, xsum[j], (2 * t + e) * 4);   // the quad that summed this column
+            if (there && c0 + c < end) {
+              store_grouped(m, r, c0 + c,
+                            finish_grouped((int32_t)((uint32_t)acc[j][2 * h + e] - (uint32_t)m.zp_w * (uint32_t)xs), (int32_t)row_term, mfp,
+                                           mexp, m));
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();   // `part` may be written again
+  }
+}
+
+template <int kTiles>
+cudaError_t launch_mma(const GroupedI8Mul& m, cudaStream_t stream) {
+  const dim3 grid((unsigned)((m.rows + 15) / 16), m.groups.count);
+  const bool ws = m.w_dtype == RUYB200_I8, xs = m.x_dtype == RUYB200_I8;
+  if (ws && xs) grouped_i8_mma_kernel<true, true, kTiles><<<grid, 32 * kMmaWarps, 0, stream>>>(m);
+  else if (ws) grouped_i8_mma_kernel<true, false, kTiles><<<grid, 32 * kMmaWarps, 0, stream>>>(m);
+  else if (xs) grouped_i8_mma_kernel<false, true, kTiles><<<grid, 32 * kMmaWarps, 0, stream>>>(m);
+  else grouped_i8_mma_kernel<false, false, kTiles><<<grid, 32 * kMmaWarps, 0, stream>>>(m);
+  return cudaGetLastError();
+}
+
+// ---- many columns per group: the 5th-generation tensor cores --------------------------------------------
+//
+// A persistent kernel: tiles of 128 weight rows x up to 256 columns of one group, tcgen05 kind::i8 with the weights on the
+// M side and the tokens on the N side, whose width follows the group (any multiple of 16), so a group of 20 columns pays
+// for 32.  Where the groups lie is only known on the device: every CTA works out the list of column tiles from the offsets
+// first (a scan in shared memory), then takes every gridDim.x-th tile.  One thread loads (128 bytes of depth per stage,
+// 128-byte swizzle), one warp issues the MMAs, eight warps drain the accumulators (two of them in tensor memory, so the
+// next tile multiplies meanwhile) and write rows of the column-major destination, 32 lanes side by side.
+//
+// Zero points.  The sums of the weights' rows (needed for a zero point of the activations) are one more MMA of 16 columns
+// against ones; the sums of the tokens (needed for one of the weights) are one more MMA of ones against the tokens, whose
+// every row then holds them: each lane finds what it needs in its own row of tensor memory, and no pass over the operands
+// and no workspace is needed.  Tiles are narrower then, to leave room in tensor memory.
+constexpr int kTileM = 128;
+constexpr int kTileK = 128;                 // bytes of depth per stage
+constexpr int kTcStages = 4;
+constexpr int kTcWBytes = kTileM * kTileK;
+constexpr int kTcXBytes = 256 * kTileK;
+constexpr int kTcStageBytes = kTcWBytes + kTcXBytes;
+constexpr int kTcOnesBytes = kTileM * kTileK;
+constexpr int kTcEpilogueWarps = 8;
+constexpr int kTcThreads = 64 + 32 * kTcEpilogueWarps;
+constexpr int kTcSmem = 1024 + kTcStages * kTcStageBytes + kTcOnesBytes;
+constexpr int kTcAccCols = 256;             // tensor-memory columns per accumulator buffer
+constexpr int kTcSumCol = 240;              // where in them the row sums are
+constexpr int kTcTokenCol = 112;            // and the tokens' sums
+
+struct TcGroupedArgs {
+  GroupedI8Mul m;
+  int64_t group_rows;   // map rows from one group's weights to the next
+  int32_t tiles_m;
+  int32_t cap;          // widest column tile, a multiple of 16
+  int32_t k_blocks;
+  uint32_t idesc;       // instruction descriptor without N
+  int32_t row_sums, token_sums;
+};
+
+__device__ __forceinline__ void tc_mma_i8(uint32_t tmem, uint32_t desc_a, uint32_t desc_b, uint32_t idesc, bool accumulate) {
+  // 128-byte swizzled, depth-contiguous tiles: rows 128 bytes apart, groups of 8 rows 1024 bytes apart
+  constexpr uint32_t kHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}"
+      ::"r"(tmem), "r"(desc_a), "r"(desc_b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kHigh)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t tc_desc(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t tc_width(int n) { return (uint32_t)(n >> 3) << 17; }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
+__device__ __forceinline__ void tc_load_32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Where a tile lies.
+struct TcTile {
+  int g, row0, c0, n;
+};
+
+// A group's columns are cut into the fewest tiles of at most `cap`, of even width.
+__device__ __forceinline__ int tiles_of(int columns, int cap) { return (columns + cap - 1) / cap; }
+
+// What the CTA has worked out from the offsets.
+struct TcPlan {
+  int first[kMaxGroups + 1];   // column tiles before each group
+  int begin[kMaxGroups];
+  int end[kMaxGroups];
+};
+
+__device__ __forceinline__ TcTile find_tile(const TcGroupedArgs& a, const TcPlan& plan, int tile) {
+  const int ct = tile / a.tiles_m;
+  int lo = 0, hi = a.m.groups.count - 1;   // the last group whose first tile is at or before ct
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (plan.first[mid] <= ct) lo = mid; else hi = mid - 1;
+  }
+  const int columns = plan.end[lo] - plan.begin[lo];
+  const int count = tiles_of(columns, a.cap);
+  const int width = ((columns + count - 1) / count + 15) / 16 * 16;
+  TcTile t;
+  t.g = lo;
+  t.row0 = (tile - ct * a.tiles_m) * kTileM;
+  t.c0 = plan.begin[lo] + (ct - plan.first[lo]) * width;
+  t.n = min(width, plan.end[lo] - t.c0);
+  return t;
+}
+
+// Copies of 16 token rows each for narrow tiles, of 64 for wider ones.
+__device__ __forceinline__ int token_box(int n) { return n <= 48 ? 16 : 64; }
+
+template <int kDstBytes>
+__global__ void __launch_bounds__(kTcThreads, 1)
+grouped_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x16,
+                     const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ TcGroupedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ TcPlan plan;
+  __shared__ __align__(8) uint64_t full[kTcStages], empty[kTcStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const GroupedI8Mul& m = a.m;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* const ones = smem + kTcStages * kTcStageBytes;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kTcStages; s++) {
+      mbarrier_init(&full[s], 1);
+      mbarrier_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbarrier_init(&acc_full[b], 1);
+      mbarrier_init(&acc_empty[b], kTcEpilogueWarps);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (a.row_sums || a.token_sums) {
+    for (int i = threadIdx.x; i < kTcOnesBytes / 16; i += kTcThreads)
+      reinterpret_cast<uint4*>(ones)[i] = make_uint4(0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u);
+  }
+  for (int g = threadIdx.x; g < m.groups.count; g += kTcThreads) group_columns(m.groups, g, m.cols, &plan.begin[g], &plan.end[g]);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 0) {
+    // exclusive scan of the groups' tile counts, 32 groups at a time
+    int before = 0;
+    for (int g0 = 0; g0 < m.groups.count; g0 += 32) {
+      const int g = g0 + lane;
+      int v = g < m.groups.count ? tiles_of(plan.end[g] - plan.begin[g], a.cap) : 0;
+      int sum = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+      }
+      if (g < m.groups.count) plan.first[g] = before + sum - v;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) plan.first[m.groups.count] = before;
+  }
+  __syncthreads();
+  const uint32_t tmem = tmem_slot;
+  const int tiles = plan.first[m.groups.count] * a.tiles_m;
+  volatile int* abortp = &abort_flag;
+
+  if (warp == 0) {
+    // ---------------- loads ----------------
+    if (lane == 0) {
+      uint32_t s = 0, ph = 0, issued = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        const TcTile t = find_tile(a, plan, tile);
+        const int box = token_box(t.n), boxes = (t.n + box - 1) / box;
+        const CUtensorMap* map_x = box == 16 ? &map_x16 : &map_x64;
+        const int row = (int)(t.g * a.group_rows + t.row0);
+        for (int kb = 0; kb < a.k_blocks; kb++) {
+          if (!mbarrier_wait(&empty[s], ph ^ 1, abortp)) {
+            if (!*abortp) atomicCAS(m.status, 0, 21);
+            *abortp = 1;
+            ok = false;
+            break;
+          }
+          uint8_t* const sw = smem + s * kTcStageBytes;
+          mbarrier_expect(&full[s], (uint32_t)(kTcWBytes + boxes * box * kTileK));
+          copy_box_2d(sw, &map_w, kb * kTileK, row, &full[s]);
+          for (int i = 0; i < boxes; i++) copy_box_2d(sw + kTcWBytes + i * box * kTileK, map_x, kb * kTileK, t.c0 + i * box, &full[s]);
+          issued++;
+          if (++s == kTcStages) { s = 0; ph ^= 1; }
+        }
+      }
+      if (!ok && issued > 0) {
+        // give copies in flight a bounded chance to land before the CTA exits
+        const uint32_t last = issued - 1;
+        for (uint32_t i = 0; i < kAsyncSpinLimit / 64 && !mbarrier_try(&full[last % kTcStages], (last / kTcStages) & 1); i++) __nanosleep(100);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMAs: the warp stays converged, one elected lane issues ----------------
+    uint32_t s = 0, ph = 0, count = 0;
+    bool ok = true;
+    const uint32_t desc0 = tc_desc(smem_addr(smem)), desc_ones = tc_desc(smem_addr(ones));
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, count++) {
+      const TcTile t = find_tile(a, plan, tile);
+      const uint32_t buf = count & 1;
+      const int width = (t.n + 15) / 16 * 16;
+      ok = __all_sync(0xffffffffu, mbarrier_wait(&acc_empty[buf], ((count >> 1) & 1) ^ 1, abortp));
+      tc_after_sync();
+      const uint32_t acc = tmem + buf * kTcAccCols;
+      for (int kb = 0; kb < a.k_blocks && ok; kb++) {
+        ok = __all_sync(0xffffffffu, mbarrier_wait(&full[s], ph, abortp));
+        if (!ok) break;
+        tc_after_sync();
+        const uint32_t dw = desc0 + s * (kTcStageBytes >> 4), dx = dw + (kTcWBytes >> 4);
+        if (tc_elect()) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const bool more = (kb | k) != 0;
+            tc_mma_i8(acc, dw + 2 * k, dx + 2 * k, a.idesc | tc_width(width), more);
+            if (a.row_sums) tc_mma_i8(acc + kTcSumCol, dw + 2 * k, desc_ones + 2 * k, a.idesc | tc_width(16), more);
+            if (a.token_sums) tc_mma_i8(acc + kTcTokenCol, desc_ones + 2 * k, dx + 2 * k, a.idesc | tc_width(width), more);
+          }
+          tc_commit(&empty[s]);
+          if (kb == a.k_blocks - 1) tc_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+        if (++s == kTcStages) { s = 0; ph ^= 1; }
+      }
+    }
+    if (!ok && lane == 0) {
+      if (!*abortp) atomicCAS(m.status, 0, 22);
+      *abortp = 1;
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int quarter = warp % 4;               // the tensor-memory lanes this warp may read
+    const int first_chunk = (warp - 2) / 4;     // two warps per quarter take the 32-column chunks in turn
+    uint32_t count = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, count++) {
+      const TcTile t = find_tile(a, plan, tile);
+      const uint32_t buf = count & 1;
+      const int r = t.row0 + quarter * 32 + lane;
+      const bool there = r < m.rows;
+      const int64_t ch = (int64_t)t.g * m.groups.channel_stride + r;
+      uint32_t add = there && m.bias ? (uint32_t)__ldg(m.bias + ch) : 0u;
+      const int32_t mfp = there && m.mfp_pc ? __ldg(m.mfp_pc + ch) : m.mfp;
+      const int32_t mexp = there && m.mexp_pc ? __ldg(m.mexp_pc + ch) : m.mexp;
+      add += (uint32_t)m.zp_x * (uint32_t)m.zp_w * (uint32_t)m.depth;
+      const bool ok = __all_sync(0xffffffffu, mbarrier_wait(&acc_full[buf], (count >> 1) & 1, abortp));
+      if (!ok) {
+        if (lane == 0) {
+          if (!*abortp) atomicCAS(m.status, 0, 23);
+          *abortp = 1;
+        }
+        break;
+      }
+      tc_after_sync();
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kTcAccCols;
+      if (a.row_sums) {
+        uint32_t sum;
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(sum) : "r"(acc + kTcSumCol) : "memory");
+        tc_load_wait();
+        add -= (uint32_t)m.zp_x * sum;
+      }
+      for (int c = 32 * first_chunk; c < t.n; c += 64) {
+        uint32_t v[32];
+        tc_load_32(acc + c, v);
+        tc_load_wait();
+        if (a.token_sums) {
+          uint32_t x[32];
+          tc_load_32(acc + kTcTokenCol + c, x);
+          tc_load_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i++) v[i] -= (uint32_t)m.zp_w * x[i];
+        }
+        if (there) {
+          char* at = (char*)m.dst + ((int64_t)(t.c0 + c) * m.dst_stride + r) * kDstBytes;
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            if (c + i < t.n) {
+              const int32_t y = finish_grouped((int32_t)v[i], (int32_t)add, mfp, mexp, m);
+              if (kDstBytes == 1) *reinterpret_cast<int8_t*>(at) = (int8_t)y;
+              else if (kDstBytes == 2) *reinterpret_cast<int16_t*>(at) = (int16_t)y;
+              else *reinterpret_cast<int32_t*>(at) = y;
+            }
+            at += m.dst_stride * kDstBytes;
+          }
+        }
+      }
+      tc_before_sync();
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&acc_empty[buf]);
+    }
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <int kDstBytes>
+cudaError_t launch_tc_variant(const CUtensorMap& w, const CUtensorMap& x16, const CUtensorMap& x64, const TcGroupedArgs& a, int grid,
+                              cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(grouped_i8_tc_kernel<kDstBytes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem);
+  if (e != cudaSuccess) return e;
+  grouped_i8_tc_kernel<kDstBytes><<<grid, kTcThreads, kTcSmem, stream>>>(w, x16, x64, a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_tc(const GroupedI8Mul& m, int sm_count, cudaStream_t stream) {
+  TcGroupedArgs a;
+  memset(&a, 0, sizeof(a));
+  a.m = m;
+  a.group_rows = m.groups.lhs_stride / m.w_stride;
+  a.tiles_m = (m.rows + kTileM - 1) / kTileM;
+  a.k_blocks = (m.depth + kTileK - 1) / kTileK;
+  a.row_sums = m.zp_x != 0;
+  a.token_sums = m.zp_w != 0;
+  a.cap = a.token_sums ? kTcTokenCol : (a.row_sums ? kTcSumCol : kTcAccCols);
+  // narrower tiles when there are too few to go round (each reads its weights again, from L2)
+  const long long active = min((long long)m.groups.count, (long long)m.cols);
+  while (a.cap > 32 && a.tiles_m * max(active, (m.cols + (long long)a.cap - 1) / a.cap) < sm_count) a.cap = (a.cap / 2 + 15) / 16 * 16;
+  // int32 accumulation, operand signedness, both depth-contiguous, M = 128
+  a.idesc = (2u << 4) | ((m.w_dtype == RUYB200_I8 ? 1u : 0u) << 7) | ((m.x_dtype == RUYB200_I8 ? 1u : 0u) << 10) | ((kTileM >> 4) << 24);
+  CUtensorMap w, x16, x64;
+  const int64_t map_rows = (m.groups.count - 1) * a.group_rows + m.rows;
+  if (!make_i8_tile_map(&w, m.w, m.depth, (int)map_rows, m.w_stride, kTileM) ||
+      !make_i8_tile_map(&x16, m.x, m.depth, m.cols, m.x_stride, 16) || !make_i8_tile_map(&x64, m.x, m.depth, m.cols, m.x_stride, 64))
+    return cudaErrorInvalidValue;
+  const int grid = sm_count;
+  if (m.dst_dtype == RUYB200_I32) return launch_tc_variant<4>(w, x16, x64, a, grid, stream);
+  if (m.dst_dtype == RUYB200_I16) return launch_tc_variant<2>(w, x16, x64, a, grid, stream);
+  return launch_tc_variant<1>(w, x16, x64, a, grid, stream);
+}
+
+// 16-byte aligned rows (the copy engine, and 16-byte loads), groups a whole number of rows apart; indices of 32 bits.
+bool aligned_layout(const GroupedI8Mul& m) {
+  if (m.depth == 0 || m.depth > (1 << 30) || m.rows > (1 << 30) || m.cols > (1 << 30)) return false;
+  if ((((uintptr_t)m.w | (uintptr_t)m.x | (uintptr_t)m.w_stride | (uintptr_t)m.x_stride) & 15) != 0) return false;
+  if (m.groups.lhs_stride % m.w_stride != 0) return false;
+  const int64_t per = m.groups.lhs_stride / m.w_stride;
+  return per <= 0x7fffffff && (m.groups.count - 1) * per + m.rows + kTileM <= 0x7fffffff;
+}
+
 }  // namespace
 
 cudaError_t launch_grouped_i8(const GroupedI8Mul& m, int sm_count, cudaStream_t stream, int* kernel) {
-  (void)sm_count;
-  *kernel = RUYB200_KERNEL_GENERIC;
-  return launch_any(m, stream);
+  if (!aligned_layout(m)) {
+    *kernel = RUYB200_KERNEL_GENERIC;
+    return launch_any(m, stream);
+  }
+  const long long active = min((long long)m.groups.count, (long long)m.cols);
+  if (m.cols <= 8 * active) {
+    *kernel = RUYB200_KERNEL_GROUPED_MMA;
+    return m.cols <= 4 * active ? launch_mma<1>(m, stream) : launch_mma<2>(m, stream);
+  }
+  *kernel = RUYB200_KERNEL_GROUPED_TC;
+  return launch_tc(m, sm_count, stream);
 }
 
 }  // namespace ruyb200
