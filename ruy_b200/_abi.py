@@ -4,6 +4,7 @@ Every structure here must stay field-for-field identical to the C header; the
 test-suite checks sizes and the exported symbol list against the header text.
 """
 import ctypes as C
+import struct
 
 ABI_VERSION = 2
 
@@ -106,6 +107,15 @@ class Q4ScalesDesc(C.Structure):
     ]
 
 
+# The same structs as byte strings, which cost a fraction of what filling ctypes structures field by field does; for calls
+# whose whole work on the device takes microseconds.  One entry per type of the clamp bounds.
+_MATRIX = "PiiiiBBBB4x"
+_MUL = {"i": "i4xi4x", "f": "f4xf4x", "d": "dd"}
+MUL_DESC_PACK = {k: struct.Struct("@" + 3 * _MATRIX + "PPPii" + v + "BBBB4x") for k, v in _MUL.items()}
+GROUPS_PACK = struct.Struct("@Pqqqii")
+Q4_SCALES_PACK = struct.Struct("@PPiiB7x")
+
+
 class CacheBlob(C.Structure):
     """ruyb200_cache_blob."""
     _fields_ = [
@@ -170,9 +180,10 @@ PROTOTYPES = {
     "ruyb200_cache_export": (C.c_int, [C.c_void_p, _P(MatrixDesc), C.c_int, C.c_void_p, _P(C.c_size_t)]),
     "ruyb200_cache_import": (C.c_int, [C.c_void_p, _P(MatrixDesc), C.c_int, C.c_void_p, C.c_size_t]),
     "ruyb200_mul_noalloc": (C.c_int, [_P(MulDesc), C.c_void_p]),
-    "ruyb200_mul_grouped_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(GroupsDesc)]),
-    "ruyb200_mul_q4_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(Q4ScalesDesc)]),
-    "ruyb200_mul_grouped_q4_async": (C.c_int, [C.c_void_p, _P(MulDesc), _P(Q4ScalesDesc), _P(GroupsDesc)]),
+    # descriptors as pointers to the structs or as the byte strings made by the *_PACK formats
+    "ruyb200_mul_grouped_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ruyb200_mul_q4_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ruyb200_mul_grouped_q4_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ruyb200_plan_create": (C.c_int, [C.c_void_p, _P(MulDesc), C.c_int, _P(C.c_void_p)]),
     "ruyb200_plan_run": (C.c_int, [C.c_void_p]),
     "ruyb200_plan_destroy": (C.c_int, [C.c_void_p]),

@@ -12,6 +12,7 @@ library, and loading fails loudly if the library has not been built.
 """
 import ctypes as C
 import enum
+import functools
 
 import numpy as np
 
@@ -78,7 +79,8 @@ class Layout:
     """ruy::Layout (ruy/matrix.h:33-51)."""
 
     def __init__(self, rows=0, cols=0, stride=0, order=Order.kColMajor):
-        self.rows, self.cols, self.stride, self.order = rows, cols, stride, Order(order)
+        self.rows, self.cols, self.stride = rows, cols, stride
+        self.order = order if type(order) is Order else Order(order)
 
 
 def make_simple_layout(rows, cols, order):
@@ -97,6 +99,9 @@ _torch_codes = {}   # torch dtype -> ruyb200_dtype, filled when the first tensor
 def _ptr_and_dtype(data):
     if data is None:
         return None, None
+    code = _torch_codes.get(data.dtype)
+    if code is not None:
+        return data.data_ptr(), code
     if _is_torch(data):
         if not _torch_codes:
             import torch
@@ -104,6 +109,17 @@ def _ptr_and_dtype(data):
         return data.data_ptr(), _torch_codes[data.dtype]
     a = data
     return a.ctypes.data, _abi.DTYPE_OF_NUMPY[a.dtype.name]
+
+
+@functools.lru_cache(maxsize=None)
+def _dtype_name(dtype):
+    return np.dtype(dtype).name
+
+
+@functools.lru_cache(maxsize=None)
+def _int_range(name):
+    info = np.iinfo(name)
+    return int(info.min), int(info.max)
 
 
 class Matrix:
@@ -114,18 +130,16 @@ class Matrix:
         self.data = data
         self.layout = layout if layout is not None else Layout()
         self.zero_point = zero_point
-        self.cache_policy = CachePolicy(cache_policy)
+        self.cache_policy = cache_policy if type(cache_policy) is CachePolicy else CachePolicy(cache_policy)
+
+    def _fields(self):
+        ptr, dt = _ptr_and_dtype(self.data)
+        lay = self.layout
+        return (ptr or 0, lay.rows, lay.cols, lay.stride, int(self.zero_point), lay.order, dt if dt is not None else 0,
+                self.cache_policy, 0)
 
     def to_desc(self):
-        ptr, dt = _ptr_and_dtype(self.data)
-        d = _abi.MatrixDesc()
-        d.data = ptr
-        d.rows, d.cols, d.stride = self.layout.rows, self.layout.cols, self.layout.stride
-        d.zero_point = int(self.zero_point)
-        d.order = int(self.layout.order)
-        d.dtype = dt if dt is not None else 0
-        d.cache_policy = int(self.cache_policy)
-        return d
+        return _abi.MatrixDesc(*self._fields())
 
 
 class MulParams:
@@ -136,8 +150,8 @@ class MulParams:
     dimension kRow (ruy/mul_params.h:228-299)."""
 
     def __init__(self, accum="int32", dst="int8"):
-        self.accum = np.dtype(accum).name
-        self.dst = np.dtype(dst).name
+        self.accum = _dtype_name(accum)
+        self.dst = _dtype_name(dst)
         self.bias = None
         self.multiplier_fixedpoint = 0
         self.multiplier_exponent = 0
@@ -146,39 +160,41 @@ class MulParams:
         if self.accum in ("float32", "float64"):
             self.clamp_min, self.clamp_max = -np.inf, np.inf
         else:
-            info = np.iinfo(self.dst)
-            self.clamp_min, self.clamp_max = int(info.min), int(info.max)
+            self.clamp_min, self.clamp_max = _int_range(self.dst)
         self.channel_dimension = ChannelDimension.kRow
         self.perchannel_buffers_capacity_rounding = 1
         self.rounding = Rounding.kFromPath
 
-    def to_desc(self):
-        p = _abi.MulParamsDesc()
-        p.bias = _ptr_and_dtype(self.bias)[0]
-        p.multiplier_fixedpoint_perchannel = _ptr_and_dtype(self.multiplier_fixedpoint_perchannel)[0]
-        p.multiplier_exponent_perchannel = _ptr_and_dtype(self.multiplier_exponent_perchannel)[0]
-        p.multiplier_fixedpoint = int(self.multiplier_fixedpoint)
-        p.multiplier_exponent = int(self.multiplier_exponent)
+    def _fields(self):
+        """The descriptor's fields, and which member of ruyb200_scalar the clamp bounds are."""
         if self.accum == "float64":
-            p.clamp_min.d = float(self.clamp_min)
-            p.clamp_max.d = float(self.clamp_max)
+            kind, lo, hi = "d", float(self.clamp_min), float(self.clamp_max)
         elif self.accum == "float32":
-            p.clamp_min.f = float(self.clamp_min)
-            p.clamp_max.f = float(self.clamp_max)
+            kind, lo, hi = "f", float(self.clamp_min), float(self.clamp_max)
         else:
-            p.clamp_min.i = int(self.clamp_min)
-            p.clamp_max.i = int(self.clamp_max)
-        p.channel_dimension = int(self.channel_dimension)
-        p.perchannel_buffers_capacity_rounding_log2 = int(self.perchannel_buffers_capacity_rounding).bit_length() - 1
-        p.accum_dtype = _abi.DTYPE_OF_NUMPY[self.accum]
-        p.rounding_mode = int(self.rounding)
+            kind, lo, hi = "i", int(self.clamp_min), int(self.clamp_max)
+        return kind, (_ptr_and_dtype(self.bias)[0] or 0, _ptr_and_dtype(self.multiplier_fixedpoint_perchannel)[0] or 0,
+                      _ptr_and_dtype(self.multiplier_exponent_perchannel)[0] or 0, int(self.multiplier_fixedpoint),
+                      int(self.multiplier_exponent), lo, hi, self.channel_dimension,
+                      int(self.perchannel_buffers_capacity_rounding).bit_length() - 1, _abi.DTYPE_OF_NUMPY[self.accum], self.rounding)
+
+    def to_desc(self):
+        kind, f = self._fields()
+        p = _abi.MulParamsDesc(*f[:5])
+        setattr(p.clamp_min, kind, f[5])
+        setattr(p.clamp_max, kind, f[6])
+        p.channel_dimension, p.perchannel_buffers_capacity_rounding_log2, p.accum_dtype, p.rounding_mode = f[7:]
         return p
 
 
 def make_desc(lhs, rhs, mul_params, dst):
-    d = _abi.MulDesc()
-    d.lhs, d.rhs, d.dst, d.params = lhs.to_desc(), rhs.to_desc(), dst.to_desc(), mul_params.to_desc()
-    return d
+    return _abi.MulDesc(lhs.to_desc(), rhs.to_desc(), dst.to_desc(), mul_params.to_desc())
+
+
+def _packed_desc(lhs, rhs, mul_params, dst):
+    """make_desc's struct as bytes."""
+    kind, f = mul_params._fields()
+    return _abi.MUL_DESC_PACK[kind].pack(*lhs._fields(), *rhs._fields(), *dst._fields(), *f)
 
 
 class Context:
@@ -302,11 +318,14 @@ class Groups:
         self.channel_stride = channel_stride
         self.scale_stride = scale_stride
 
-    def to_desc(self):
+    def _fields(self):
         ptr, dt = _ptr_and_dtype(self.offsets)
         if dt != _abi.I32:
             raise TypeError("Groups.offsets must be int32")
-        return _abi.GroupsDesc(ptr, self.lhs_stride, self.channel_stride, self.scale_stride, max(0, len(self.offsets) - 1))
+        return ptr, self.lhs_stride, self.channel_stride, self.scale_stride, max(0, len(self.offsets) - 1), 0
+
+    def to_desc(self):
+        return _abi.GroupsDesc(*self._fields())
 
 
 class Q4Scales:
@@ -319,12 +338,15 @@ class Q4Scales:
         self.stride = stride
         self.zero_points = zero_points
 
-    def to_desc(self):
+    def _fields(self):
         ptr, dt = _ptr_and_dtype(self.scales)
         zp, zdt = _ptr_and_dtype(self.zero_points)
         if zdt not in (None, _abi.I8):
             raise TypeError("Q4Scales.zero_points must be int8")
-        return _abi.Q4ScalesDesc(ptr, zp, self.block, self.stride, dt if dt is not None else 0)
+        return ptr or 0, zp or 0, self.block, self.stride, dt if dt is not None else 0
+
+    def to_desc(self):
+        return _abi.Q4ScalesDesc(*self._fields())
 
 
 class Q4Matrix:
@@ -337,30 +359,34 @@ class Q4Matrix:
         self.scales = scales
         self.signed = signed
 
-    def to_desc(self):
+    def _fields(self):
         lay = self.layout
-        return _abi.MatrixDesc(_ptr_and_dtype(self.data)[0], lay.rows, lay.cols, lay.stride, 0, lay.order,
-                               _abi.I4 if self.signed else _abi.U4, 0, 0)
+        return (_ptr_and_dtype(self.data)[0] or 0, lay.rows, lay.cols, lay.stride, 0, lay.order, _abi.I4 if self.signed else _abi.U4,
+                0, 0)
+
+    def to_desc(self):
+        return _abi.MatrixDesc(*self._fields())
 
 
 def mul_grouped_async(lhs, rhs, mul_params, context, dst, groups):
     """ruyb200_mul_grouped_async: the 8-bit mul of every group's weights with that group's columns, in one launch.  `lhs`
     describes the first group's weights.  Stream-ordered, device-resident operands."""
-    d, g = make_desc(lhs, rhs, mul_params, dst), groups.to_desc()
-    _check(lib().ruyb200_mul_grouped_async(context._h, C.byref(d), C.byref(g)), "ruyb200_mul_grouped_async")
+    _check(lib().ruyb200_mul_grouped_async(context._h, _packed_desc(lhs, rhs, mul_params, dst), _abi.GROUPS_PACK.pack(*groups._fields())),
+           "ruyb200_mul_grouped_async")
 
 
 def mul_q4_async(lhs, rhs, mul_params, context, dst):
     """ruyb200_mul_q4_async: 4-bit weights (a Q4Matrix) times a few columns of float, half or bfloat16 activations.
     Stream-ordered, device-resident operands."""
-    d, q = make_desc(lhs, rhs, mul_params, dst), lhs.scales.to_desc()
-    _check(lib().ruyb200_mul_q4_async(context._h, C.byref(d), C.byref(q)), "ruyb200_mul_q4_async")
+    _check(lib().ruyb200_mul_q4_async(context._h, _packed_desc(lhs, rhs, mul_params, dst), _abi.Q4_SCALES_PACK.pack(*lhs.scales._fields())),
+           "ruyb200_mul_q4_async")
 
 
 def mul_grouped_q4_async(lhs, rhs, mul_params, context, dst, groups):
     """ruyb200_mul_grouped_q4_async: mul_q4_async with groups."""
-    d, q, g = make_desc(lhs, rhs, mul_params, dst), lhs.scales.to_desc(), groups.to_desc()
-    _check(lib().ruyb200_mul_grouped_q4_async(context._h, C.byref(d), C.byref(q), C.byref(g)), "ruyb200_mul_grouped_q4_async")
+    _check(lib().ruyb200_mul_grouped_q4_async(context._h, _packed_desc(lhs, rhs, mul_params, dst),
+                                              _abi.Q4_SCALES_PACK.pack(*lhs.scales._fields()), _abi.GROUPS_PACK.pack(*groups._fields())),
+           "ruyb200_mul_grouped_q4_async")
 
 
 def cache_blob_info(blob):

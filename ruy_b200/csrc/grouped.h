@@ -1,6 +1,8 @@
 // Internal declarations of the muls with weights in groups and with weights of 4 bits (grouped.cu, grouped_i8.cu, q4.cu).
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ruyb200 {
@@ -69,6 +71,19 @@ struct Q4Mul {
   int* status;
 };
 cudaError_t launch_q4(const Q4Mul& m, int sm_count, cudaStream_t stream, int* kernel);
+
+// Raises a kernel's limit of dynamic shared memory, once per device and kernel (`done`, one entry per device); contexts on
+// several threads may get here together, and the call may repeat.
+constexpr int kMaxDevices = 64;
+inline cudaError_t allow_smem(const void* kernel, size_t bytes, std::atomic<bool>* done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (known && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && known) done[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
 
 // Accumulator (zero points taken care of, bias not yet added) -> destination value before the narrowing cast.
 __device__ __forceinline__ int32_t finish_grouped(int32_t acc, int32_t bias, int32_t mfp, int32_t mexp, const GroupedI8Mul& m) {

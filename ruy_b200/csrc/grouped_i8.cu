@@ -534,7 +534,8 @@ grouped_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 template <int kDstBytes>
 cudaError_t launch_tc_variant(const CUtensorMap& w, const CUtensorMap& x16, const CUtensorMap& x64, const TcGroupedArgs& a, int grid,
                               cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(grouped_i8_tc_kernel<kDstBytes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem);
+  static std::atomic<bool> allowed[kMaxDevices];
+  const cudaError_t e = allow_smem((const void*)grouped_i8_tc_kernel<kDstBytes>, kTcSmem, allowed);
   if (e != cudaSuccess) return e;
   grouped_i8_tc_kernel<kDstBytes><<<grid, kTcThreads, kTcSmem, stream>>>(w, x16, x64, a);
   return cudaGetLastError();

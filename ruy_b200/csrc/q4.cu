@@ -584,7 +584,8 @@ cudaError_t launch_staged(const Q4Args& a, cudaStream_t stream) {
   if (!make_i8_tile_map(&map, m.w, (m.depth + 1) / 2, (int)map_rows, m.w_stride / 2, kRows)) return cudaErrorInvalidValue;
   static_assert(kMaxTiles * 8 * kRows * 4 <= kStages<kType> * kStageBytes, "the sums of a pass fit into the ring");
   const size_t smem = 1024 + (size_t)kStages<kType> * kStageBytes + 2 * (size_t)a.x_bytes;
-  cudaError_t e = cudaFuncSetAttribute(q4_kernel<kType, kPer, kMaxTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<bool> allowed[kMaxDevices];   // smem is the same for every launch of an instantiation
+  const cudaError_t e = allow_smem((const void*)q4_kernel<kType, kPer, kMaxTiles>, smem, allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

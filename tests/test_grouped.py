@@ -30,6 +30,32 @@ def test_struct_layout_matches_c(tmp_path):
                    _abi.Q4ScalesDesc.block.offset, _abi.Q4ScalesDesc.dtype.offset, _abi.F16, _abi.BF16, _abi.I4, _abi.U4]
 
 
+@pytest.mark.parametrize("accum,lo,hi", [("int32", -100, 101), ("float32", -1.5, float("inf")), ("float64", 2.0 ** -60, 3.0)])
+def test_packed_descriptors_are_the_structs(accum, lo, hi):
+    t = {"int32": np.int8, "float32": np.float32, "float64": np.float64}[accum]
+    a, b, c = np.zeros((4, 6), t), np.zeros((5, 6), t), np.zeros((5, 7), t)
+    lhs = rb.Matrix(a, rb.Layout(4, 5, 6, RowMajor), -3, rb.CachePolicy.kAlwaysCache)
+    rhs, dst = rb.Matrix(b, rb.Layout(5, 5, 6, ColMajor), 17), rb.Matrix(c, rb.Layout(4, 5, 7, ColMajor), 2)
+    p = rb.MulParams(accum, t)
+    p.bias, p.multiplier_fixedpoint_perchannel, p.multiplier_exponent_perchannel = a, b, c
+    p.multiplier_fixedpoint, p.multiplier_exponent, p.clamp_min, p.clamp_max = 5, -6, lo, hi
+    p.channel_dimension, p.perchannel_buffers_capacity_rounding, p.rounding = rb.ChannelDimension.kCol, 8, rb.Rounding.kX86
+    from ruy_b200 import api
+    packed = _abi.MulDesc.from_buffer_copy(api._packed_desc(lhs, rhs, p, dst))
+    assert len(api._packed_desc(lhs, rhs, p, dst)) == C.sizeof(_abi.MulDesc)
+    plain = rb.make_desc(lhs, rhs, p, dst)
+
+    def values(s):
+        return [values(getattr(s, n)) if isinstance(getattr(s, n), C.Structure) else
+                getattr(getattr(s, n), {"int32": "i", "float32": "f", "float64": "d"}[accum]) if isinstance(getattr(s, n), C.Union) else
+                getattr(s, n) for n, _ in s._fields_]
+    assert values(packed) == values(plain)
+    scales = rb.Q4Scales(np.zeros(8, np.float16), 64, 9, np.zeros(8, np.int8))
+    assert bytes(scales.to_desc()) == _abi.Q4_SCALES_PACK.pack(*scales._fields())
+    groups = rb.Groups(np.zeros(8, np.int32), 64, 9, 2 ** 40)
+    assert bytes(groups.to_desc()) == _abi.GROUPS_PACK.pack(*groups._fields())
+
+
 class _NoContext:
     _h = None
 
