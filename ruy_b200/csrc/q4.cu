@@ -112,7 +112,8 @@ cudaError_t launch_any(const Q4Mul& m, cudaStream_t stream) {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16 * kWarps;          // weight rows per CTA
-constexpr int kSlab = 256;                  // depth per ring stage
+constexpr int kSlabShift = 8;
+constexpr int kSlab = 1 << kSlabShift;      // depth per ring stage
 constexpr int kSteps = kSlab / 32;
 constexpr int kStageBytes = kRows * kSlab / 2;
 constexpr int kMaxSplit = 8;                // CTAs of a cluster that share the depth (the portable cluster size)
@@ -123,6 +124,7 @@ struct Q4Args {
   int32_t x_bytes;      // shared memory for the activations of a segment
   int32_t room;         // columns per pass
   int32_t split;        // CTAs per cluster
+  int32_t pass_lanes;   // CTAs that share a group's passes
   int32_t slabs_per;    // slabs of depth per CTA
   int32_t blocks;       // per row
   int32_t block_steps;  // steps per block
@@ -150,45 +152,53 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], bool fresh, uint32_t a0
   }
 }
 
-// What is added to the widened elements of one row: minus the number that the widening brings in, minus 8 for signed
-// weights (whose sign bit the widening flips), minus the zero point, twice.  f16 has a second pair for the elements that
-// come from the upper half of a byte.
+// Widening.  Masks leave a 4-bit number q in the low bits of a 16-bit half, or four bits further up, and q - z comes out of
+// one multiply-add, exactly (`flip` has bit 3 of every element set for signed weights, whose z is 8 larger then):
+//   f16   the significand of 1024 with q in its low bits reads as 1024 + q, four bits up as 1024 + 16 q
+//   bf16  the significand of 128 with q in its low bits reads as 128 + q; four bits up there is no room, but there the bare
+//         bits (a subnormal number, or one of the smallest normal ones) read as 16 q * 2**-133, which times 2**127 is q / 4.
+//         The whole product is formed in quarters, and the sums are multiplied by kUnit at the end
+// One shift per word serves both halves of the bytes.
+template <int kType>
+constexpr float kUnit = kType == kHalf ? 1.f : 4.f;
+
+// The addends of one row: for elements from the lower and from the upper half of a byte, each twice.
 template <int kType>
 __device__ __forceinline__ uint32_t low_offset(int z) {
   if (kType == kHalf) {
     const __half2 v = __half2half2(__int2half_rn(-(1024 + z)));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  const __nv_bfloat162 v = __bfloat162bfloat162(__int2bfloat16_rn(-(128 + z)));
+  const __nv_bfloat162 v = __float2bfloat162_rn(-0.25f * (float)(128 + z));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+template <int kType>
 __device__ __forceinline__ uint32_t high_offset(int z) {
-  const __half2 v = __half2half2(__int2half_rn(-(64 + z)));
+  if (kType == kHalf) {
+    const __half2 v = __half2half2(__int2half_rn(-(64 + z)));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __nv_bfloat162 v = __float2bfloat162_rn(-0.25f * (float)z);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight 4-bit elements -> four pairs (0,4), (1,5), (2,6), (3,7).  A 4-bit number placed in the low bits of the significand
-// of 128 (bf16: one step is 1) or 1024 (f16: one step is 1, four bits up it is 16) reads as that number plus it; the
-// addition of the offset is exact.  `flip` has bit 3 of every element set for signed weights.
+// Eight 4-bit elements -> four pairs (0,4), (1,5), (2,6), (3,7).
 template <int kType>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t flip, uint32_t low, uint32_t high, uint32_t (&v)[4]) {
-  if (kType == kHalf) {
-    const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint32_t u = w >> (8 * i);
+  for (int i = 0; i < 2; i++) {
+    const uint32_t u = w >> (8 * i);
+    if (kType == kHalf) {
       const uint32_t a = (u & 0x000f000fu) ^ (0x64006400u | (flip & 0x000f000fu)), b = (u & 0x00f000f0u) ^ (0x64006400u | (flip & 0x00f000f0u));
       const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&low));
-      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, *reinterpret_cast<const __half2*>(&high));
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(0.0625f), *reinterpret_cast<const __half2*>(&high));
       v[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
       v[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t a = ((w >> (4 * i)) & 0x000f000fu) ^ (0x43004300u | (flip & 0x000f000fu));
-      const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&low));
-      v[i] = *reinterpret_cast<const uint32_t*>(&x);
+    } else {
+      const uint32_t a = (u & 0x000f000fu) ^ (0x43004300u | (flip & 0x000f000fu)), b = (u & 0x00f000f0u) ^ (flip & 0x00f000f0u);
+      const uint32_t quarter = 0x3e803e80u, large = 0x7f007f00u;   // 1/4 and 2**127, twice
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[2 * i]) : "r"(a), "r"(quarter), "r"(low));
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[2 * i + 1]) : "r"(b), "r"(large), "r"(high));
     }
   }
 }
@@ -254,23 +264,24 @@ struct Carried {
   static constexpr int kSlabColumns = kItems * kThreads / (kSlab / 8);
   X8<kType> x[kItems];
 
-  __device__ __forceinline__ void load(const Q4Args& a, int slabs, int c0, int n, int k0) {
-    const int per = slabs * (kSlab / 8), items = n * per;
+  // A segment of 1 << shift slabs from depth k0 on; what lies at or beyond `end` (whole slabs) is left out.
+  __device__ __forceinline__ void load(const Q4Args& a, int shift, int c0, int n, int k0, int end) {
+    const int lg = shift + kSlabShift - 3;
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
       const int i = threadIdx.x + u * kThreads;
-      const int c = i / per, p = i - c * per;
-      if (i < items) load_x8<kType>(a, c0 + c, k0 + 8 * p, x[u]);
+      const int c = i >> lg, k = k0 + 8 * (i - (c << lg));
+      if (c < n && k < end) load_x8<kType>(a, c0 + c, k, x[u]);
     }
   }
 
-  __device__ __forceinline__ void store(uint8_t* xs, int pitch, int slabs, int n) const {
-    const int per = slabs * (kSlab / 8), items = n * per;
+  __device__ __forceinline__ void store(uint8_t* xs, int pitch, int shift, int n) const {
+    const int lg = shift + kSlabShift - 3;
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
       const int i = threadIdx.x + u * kThreads;
-      const int c = i / per, p = i - c * per;
-      if (i >= items) break;
+      const int c = i >> lg, p = i - (c << lg);
+      if (c >= n) break;
       uint8_t* const to = xs + c * pitch + 16 * p;
       const uint32_t (&v)[sizeof(x[u].v) / 4] = x[u].v;
       if constexpr (kType == kFloat3) {
@@ -370,7 +381,8 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
   constexpr int kChains = kTiles == 1 ? 2 : 1;    // independent accumulators, so that an MMA need not wait for the last one
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, t = lane & 3, quad = lane >> 2;
   const int used = n * kPieces;
-  const int seg_slabs = min(max(slab1 - slab0, 1), Carried<kType>::kSlabColumns / n);
+  const int seg_shift = 31 - __clz(Carried<kType>::kSlabColumns / n);   // slabs per segment: as many as fit, a power of two
+  const int seg_slabs = 1 << seg_shift;
   const int pitch = seg_slabs * kSlab * 2 + 64;   // 64 modulo 128: a quarter-warp's fragment loads hit every bank once
   const uint32_t flip = a.m.w_signed ? 0x88888888u : 0u;
   const int base_z = a.m.w_signed ? 8 : 0;
@@ -399,24 +411,31 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
   fetch_scales<kPer>(a, row_at, row_there && slab0 < slab1, slab0, next[0]);
   fetch_scales<kPer>(a, row_at, row_there && slab0 + 1 < slab1, slab0 + 1, next[1]);
   Carried<kType> carried;
-  carried.load(a, min(seg_slabs, slab1 - slab0), c0, n, slab0 * kSlab);
+  carried.load(a, seg_shift, c0, n, slab0 * kSlab, slab1 * kSlab);
+  uint32_t low[kPer], high[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    low[i] = low_offset<kType>(base_z);
+    high[i] = high_offset<kType>(base_z);
+  }
   int buffer = 0;
   for (int s0 = slab0; s0 < slab1; s0 += seg_slabs, buffer ^= 1) {
     const int count = min(seg_slabs, slab1 - s0);
-    carried.store(xs + buffer * a.x_bytes, pitch, count, n);
+    carried.store(xs + buffer * a.x_bytes, pitch, seg_shift, n);
     // one barrier per segment: whoever fills a buffer again has passed the barrier of the segment in between, which
     // every warp reaches after its last load from that buffer
     __syncthreads();
-    if (s0 + seg_slabs < slab1) carried.load(a, min(seg_slabs, slab1 - s0 - seg_slabs), c0, n, (s0 + seg_slabs) * kSlab);
+    if (s0 + seg_slabs < slab1) carried.load(a, seg_shift, c0, n, (s0 + seg_slabs) * kSlab, slab1 * kSlab);
     const uint8_t* xb = xs + buffer * a.x_bytes;
     for (int s = s0; s < s0 + count; s++, xb += kSteps * 64) {
       float scale[kPer];
-      uint32_t low[kPer], high[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
         scale[i] = scale_value(a.m, next[0].scale[i]);
-        low[i] = low_offset<kType>(base_z + next[0].zero[i]);
-        high[i] = kType == kHalf ? high_offset(base_z + next[0].zero[i]) : 0u;
+        if (a.m.zero_points) {
+          low[i] = low_offset<kType>(base_z + next[0].zero[i]);
+          high[i] = high_offset<kType>(base_z + next[0].zero[i]);
+        }
       }
       next[0] = next[1];
       fetch_scales<kPer>(a, row_at, row_there && s + 2 < slab1, s + 2, next[1]);
@@ -433,10 +452,8 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
         if (a.m.zero_points) {
           l0 = __shfl_sync(0xffffffffu, low[i], from0 + half);
           l1 = __shfl_sync(0xffffffffu, low[i], from1 + half);
-          if (kType == kHalf) {
-            h0 = __shfl_sync(0xffffffffu, high[i], from0 + half);
-            h1 = __shfl_sync(0xffffffffu, high[i], from1 + half);
-          }
+          h0 = __shfl_sync(0xffffffffu, high[i], from0 + half);
+          h1 = __shfl_sync(0xffffffffu, high[i], from1 + half);
         }
         const uint32_t w0 = *reinterpret_cast<const uint32_t*>(wbase + ((b ^ quad) << 4));
         const uint32_t w1 = *reinterpret_cast<const uint32_t*>(wbase + ((b ^ quad) << 4) + 1024);
@@ -535,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
   const int slab0 = min(rank * a.slabs_per, slabs), slab1 = min(slab0 + a.slabs_per, slabs);
   volatile int* abortp = &abort_flag;
   Ring ring = {full, empty, data, &map, (int)(g * a.group_rows + row0), 0, 0, 0, 0, true};
-  for (int c0 = begin; c0 < end; c0 += a.room) {
+  // a long group's passes are shared out along the grid's third axis
+  for (int c0 = begin + (int)blockIdx.z * a.room; c0 < end; c0 += (int)gridDim.z * a.room) {
     const int n = min(a.room, end - c0);
     const int tiles = (n * kPieces + 7) / 8;
     if (kMaxTiles <= 2) {
@@ -560,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
           v += a.split > 1 ? load_of_rank(at, s) : *at;
         }
       }
-      if (row0 + r < a.m.rows) store_q4(a.m, g, row0 + r, c0 + c, v);
+      if (row0 + r < a.m.rows) store_q4(a.m, g, row0 + r, c0 + c, v * kUnit<kType>);
     }
     asm volatile("fence.proxy.async;" ::: "memory");            // the copy engine writes where `part` was
     if (a.split > 1) cluster_barrier(); else __syncthreads();   // `part` may be overwritten, or its CTA gone
@@ -589,7 +607,7 @@ cudaError_t launch_staged(const Q4Args& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(((long long)m.rows + kRows - 1) / kRows * a.split), m.groups.count);
+  cfg.gridDim = dim3((unsigned)(((long long)m.rows + kRows - 1) / kRows * a.split), m.groups.count, a.pass_lanes);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -647,6 +665,7 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
   a.slabs_per = (slabs + a.split - 1) / a.split;
   // the largest segment: its rows, and the padding between them
   const int slab_columns = pieces == 3 ? Carried<kFloat3>::kSlabColumns : Carried<kBf16>::kSlabColumns;
+  a.pass_lanes = (int)min(4ll, (m.cols + (long long)a.room - 1) / a.room);
   a.x_bytes = pieces * (slab_columns * kSlab * 2 + a.room * 64);
   if (pieces == 3) return few ? launch_by_block<kFloat3, 2>(a, stream) : launch_by_block<kFloat3, 6>(a, stream);
   if (m.x_dtype == RUYB200_F16) return few ? launch_by_block<kHalf, 2>(a, stream) : launch_by_block<kHalf, 4>(a, stream);
