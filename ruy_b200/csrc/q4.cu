@@ -337,6 +337,18 @@ __device__ __forceinline__ float scale_value(const Q4Mul& m, uint32_t raw) {
   return __half2float(__ushort_as_half((unsigned short)raw));
 }
 
+// Loads by shared-memory address; volatile, so that they stay behind the waits that precede them.
+__device__ __forceinline__ uint32_t load_shared(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_shared4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
 // The ring of slabs.  Warp 0 refills it between its own multiplications, one slab behind the consumption so that the
 // other warps need not keep exact step with it.
 struct Ring {
@@ -387,10 +399,11 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
   const uint32_t flip = a.m.w_signed ? 0x88888888u : 0u;
   const int base_z = a.m.w_signed ? 8 : 0;
   // MMA columns are independent of one another: those without an activation multiply column 0 again and are not stored
-  int xat[kTiles];
+  uint32_t xat[kTiles];
 #pragma unroll
-  for (int j = 0; j < kTiles; j++) xat[j] = (8 * j + quad < used ? 8 * j + quad : 0) * pitch + 16 * t;
-  const uint8_t* const wat = ring.data + (warp * 16 + quad) * 128 + 4 * t;
+  for (int j = 0; j < kTiles; j++) xat[j] = smem_addr(xs) + (uint32_t)((8 * j + quad < used ? 8 * j + quad : 0) * pitch + 16 * t);
+  // row `quad` of the warp's 16 in the first stage; the swizzle puts the 16 bytes of step b at b ^ (row % 8)
+  const uint32_t wat = smem_addr(ring.data) + (uint32_t)((warp * 16 + quad) * 128 + (quad << 4) + 4 * t);
   // where this lane fetches scales, and from which lanes it takes those of its rows `quad` and `quad` + 8
   const int my_row = row0 + warp * 16 + (lane >> 1);
   const bool row_there = my_row < a.m.rows;
@@ -426,7 +439,7 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
     // every warp reaches after its last load from that buffer
     __syncthreads();
     if (s0 + seg_slabs < slab1) carried.load(a, seg_shift, c0, n, (s0 + seg_slabs) * kSlab, slab1 * kSlab);
-    const uint8_t* xb = xs + buffer * a.x_bytes;
+    uint32_t xb = (uint32_t)(buffer * a.x_bytes);
     for (int s = s0; s < s0 + count; s++, xb += kSteps * 64) {
       float scale[kPer];
 #pragma unroll
@@ -444,26 +457,25 @@ __device__ __forceinline__ void multiply_pass(const Q4Args& a, Ring& ring, uint8
         ring_gave_up(a, ring, 11, abort_flag);
         break;
       }
-      const uint8_t* const wbase = wat + ring.stage * kStageBytes;
+      const uint32_t wbase = wat + ring.stage * kStageBytes;
+      uint32_t l0 = low[0], l1 = low[0], h0 = high[0], h1 = high[0];
 #pragma unroll
       for (int b = 0; b < kSteps; b++) {
         const int i = (b & 3) / kFlush, half = b >> 2, chain = kChains == 2 ? 1 : 0;
-        uint32_t l0 = low[0], l1 = low[0], h0 = high[0], h1 = high[0];
-        if (a.m.zero_points) {
+        if (b % kFlush == 0 && a.m.zero_points) {   // a block's zero points
           l0 = __shfl_sync(0xffffffffu, low[i], from0 + half);
           l1 = __shfl_sync(0xffffffffu, low[i], from1 + half);
           h0 = __shfl_sync(0xffffffffu, high[i], from0 + half);
           h1 = __shfl_sync(0xffffffffu, high[i], from1 + half);
         }
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(wbase + ((b ^ quad) << 4));
-        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(wbase + ((b ^ quad) << 4) + 1024);
+        const uint32_t w0 = load_shared(wbase ^ (b << 4)), w1 = load_shared((wbase ^ (b << 4)) + 1024);
         uint32_t v0[4], v1[4];
         widen<kType>(w0, flip, l0, h0, v0);
         widen<kType>(w1, flip, l1, h1, v1);
         const bool fresh = b % kFlush == 0;
 #pragma unroll
         for (int j = 0; j < kTiles; j++) {
-          const uint4 x = *reinterpret_cast<const uint4*>(xb + xat[j] + b * 64);
+          const uint4 x = load_shared4(xat[j] + xb + b * 64);
           mma_16816<kType>(acc[0][j], fresh, v0[0], v1[0], v0[1], v1[1], x.x, x.y);
           mma_16816<kType>(acc[chain][j], fresh && chain != 0, v0[2], v1[2], v0[3], v1[3], x.z, x.w);
         }
