@@ -244,6 +244,8 @@ struct TcGroupedArgs {
   int32_t k_blocks;
   uint32_t idesc;       // instruction descriptor without N
   int32_t row_sums, token_sums;
+  int32_t clamp;        // the clamp is tighter than an 8-bit destination's type, or the destination is wider
+  int32_t dst_words;    // 8-bit destinations: four rows of a column are an aligned word
 };
 
 template <bool kPair>
@@ -354,6 +356,19 @@ __device__ __forceinline__ TcTile find_tile(const TcGroupedArgs& a, const TcPlan
 
 // Copies of 16 token rows each for narrow tiles, of 64 for wider ones.
 __device__ __forceinline__ int token_box(int n) { return n <= 48 ? 16 : 64; }
+
+// Four values within the range of int8 or uint8, or to be saturated to it, as bytes.
+__device__ __forceinline__ uint32_t narrow4(const int32_t* v, uint8_t dtype) {
+  uint32_t high, all;
+  if (dtype == RUYB200_U8) {
+    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(v[3]), "r"(v[2]), "r"(0u));
+    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(v[1]), "r"(v[0]), "r"(high));
+  } else {
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(v[3]), "r"(v[2]), "r"(0u));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(v[1]), "r"(v[0]), "r"(high));
+  }
+  return all;
+}
 
 template <int kDstBytes, bool kPair>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -520,13 +535,21 @@ grouped_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     for (int tile = unit; tile < tiles; tile += units, count++) {
       const TcTile t = find_tile<kPair>(a, plan, tile);
       const uint32_t buf = count & 1;
-      const int r = t.row0 + (int)rank * kTileM + quarter * 32 + lane;
+      const int row_base = t.row0 + (int)rank * kTileM + quarter * 32, r = row_base + lane;
       const bool there = r < m.rows;
       const int64_t ch = (int64_t)t.g * m.groups.channel_stride + r;
       uint32_t add = there && m.bias ? (uint32_t)__ldg(m.bias + ch) : 0u;
       const int32_t mfp = there && m.mfp_pc ? __ldg(m.mfp_pc + ch) : m.mfp;
       const int32_t mexp = there && m.mexp_pc ? __ldg(m.mexp_pc + ch) : m.mexp;
       add += (uint32_t)m.zp_x * (uint32_t)m.zp_w * (uint32_t)m.depth;
+      // When every shift of the warp is 32 or more, requantising is a multiply-add whose high word is shifted on, and the
+      // destination's zero point rides in the rounding term where it cannot overflow there.
+      const int shift = 31 - mexp;
+      const bool high_word = kDstBytes != 4 && !m.rounding_x86 && __all_sync(0xffffffffu, shift >= 32 && shift <= 62);
+      const bool fold_zp = shift <= 45 && m.zp_dst > -32768 && m.zp_dst < 32768;
+      const long long rounding = (1ll << ((shift - 1) & 63)) + (fold_zp ? (long long)m.zp_dst * (1ll << (shift & 63)) : 0ll);
+      const int32_t late_zp = fold_zp ? 0 : m.zp_dst;
+      const int shift_high = (shift - 32) & 31;
       const bool ok = __all_sync(0xffffffffu, mbarrier_wait(&acc_full[buf], (count >> 1) & 1, abortp));
       if (!ok) {
         if (lane == 0) {
@@ -554,15 +577,38 @@ grouped_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 #pragma unroll
           for (int i = 0; i < 32; i++) v[i] -= (uint32_t)m.zp_w * x[i];
         }
-        if (there) {
+        int32_t y[32];
+        if (kDstBytes != 4 && high_word) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            const long long p = (long long)(int32_t)(v[i] + add) * (long long)mfp + rounding;
+            y[i] = (int32_t)((uint32_t)((int32_t)(p >> 32) >> shift_high) + (uint32_t)late_zp);
+            if (a.clamp) y[i] = max(min(y[i], m.clamp_max), m.clamp_min);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i++) y[i] = finish_grouped((int32_t)v[i], (int32_t)add, mfp, mexp, m);
+        }
+        if (kDstBytes == 1 && a.dst_words && row_base + 32 <= m.rows) {   // uniform over the warp
+          // Four lanes turn their four rows x four columns of bytes round, so that each stores four rows of one column.
+          const int q = lane & 3;
+          char* at = (char*)m.dst + (int64_t)(t.c0 + c + q) * m.dst_stride + row_base + (lane & ~3);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            uint32_t w = narrow4(y + i, m.dst_dtype);
+            w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), (q & 1) ? 0x3715 : 0x6240);
+            w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2), (q & 2) ? 0x3276 : 0x5410);
+            if (c + i + q < t.n) *reinterpret_cast<uint32_t*>(at) = w;
+            at += 4 * m.dst_stride;
+          }
+        } else if (there) {
           char* at = (char*)m.dst + ((int64_t)(t.c0 + c) * m.dst_stride + r) * kDstBytes;
 #pragma unroll
           for (int i = 0; i < 32; i++) {
             if (c + i < t.n) {
-              const int32_t y = finish_grouped((int32_t)v[i], (int32_t)add, mfp, mexp, m);
-              if (kDstBytes == 1) *reinterpret_cast<int8_t*>(at) = (int8_t)y;
-              else if (kDstBytes == 2) *reinterpret_cast<int16_t*>(at) = (int16_t)y;
-              else *reinterpret_cast<int32_t*>(at) = y;
+              if (kDstBytes == 1) *reinterpret_cast<int8_t*>(at) = (int8_t)y[i];
+              else if (kDstBytes == 2) *reinterpret_cast<int16_t*>(at) = (int16_t)y[i];
+              else *reinterpret_cast<int32_t*>(at) = y[i];
             }
             at += m.dst_stride * kDstBytes;
           }
@@ -677,6 +723,11 @@ cudaError_t launch_tc(const GroupedI8Mul& m, int sm_count, cudaStream_t stream) 
   // int32 accumulation, operand signedness, both depth-contiguous, M = 128 or, of a pair, 256
   a.idesc = (2u << 4) | ((m.w_dtype == RUYB200_I8 ? 1u : 0u) << 7) | ((m.x_dtype == RUYB200_I8 ? 1u : 0u) << 10) |
             ((uint32_t)((pair ? 2 * kTileM : kTileM) >> 4) << 24);
+  // the saturating narrowing of the word stores clamps to the whole type by itself
+  a.dst_words = (((uintptr_t)m.dst | (uintptr_t)m.dst_stride) & 3) == 0;
+  const bool whole = (m.dst_dtype == RUYB200_I8 && m.clamp_min == -128 && m.clamp_max == 127) ||
+                     (m.dst_dtype == RUYB200_U8 && m.clamp_min == 0 && m.clamp_max == 255);
+  a.clamp = !(whole && a.dst_words && m.rows % 32 == 0);
   CUtensorMap w, x16, x64;
   const int64_t map_rows = (m.groups.count - 1) * a.group_rows + m.rows;
   if (!make_i8_tile_map(&w, m.w, m.depth, (int)map_rows, m.w_stride, kTileM) ||
