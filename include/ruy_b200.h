@@ -251,7 +251,8 @@ RUYB200_API int ruyb200_mul_noalloc(const ruyb200_mul_desc* desc, void* cuda_str
  *
  * All three calls are stream-ordered like ruyb200_mul_async: they validate, enqueue on the context's stream and return
  * without synchronizing.  Every pointer must be device (or managed) memory of the context's device.  They allocate
- * nothing and use no scratch memory, so they may be captured into CUDA graphs, any number of which may run at once.
+ * nothing and use no scratch memory, so they may be captured into CUDA graphs, any number of which may run at once (make
+ * the first call with a combination of types before a capture: it loads the kernel).
  * Device-side lists (offsets, zero points) are read when the kernel runs; nothing of them is read on the host.
  *
  * ruyb200_groups: column c of rhs and dst belongs to group g when offsets[g] <= c < offsets[g + 1].  The LHS of group g
@@ -259,7 +260,8 @@ RUYB200_API int ruyb200_mul_noalloc(const ruyb200_mul_desc* desc, void* cuda_str
  * the first ones (0: all groups share them), its scales and zero points scale_stride * g entries after the first ones.
  * offsets is int32[count + 1] in device memory and should not decrease.  Columns outside every group are left as they
  * were; an entry outside [0, cols] counts as the nearer end of that range, and a group that ends before it begins is
- * empty.  At most 1024 groups. */
+ * empty; a column that offsets which do decrease give to several groups gets the result of any of them.  At most 1024
+ * groups. */
 typedef struct ruyb200_groups {
   const int32_t* offsets;
   int64_t lhs_stride;

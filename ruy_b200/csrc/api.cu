@@ -1579,6 +1579,7 @@ int ctx_fail(int status, const char* msg) { return fail(status, "%s", msg); }
 int ctx_validate(const ruyb200_mul_desc* d) { return validate_desc(d); }
 bool ptr_on_device(const void* p) { return is_device_pointer(p); }
 bool ctx_trace(ruyb200_ctx* ctx) { return ctx->trace; }
+bool ctx_forces_generic(ruyb200_ctx* ctx) { return ctx->force_kernel == RUYB200_KERNEL_GENERIC; }
 int ctx_rounding_is_x86(ruyb200_ctx* ctx, int rounding_mode) {
   if (rounding_mode == RUYB200_ROUNDING_X86) return 1;
   if (rounding_mode == RUYB200_ROUNDING_REFERENCE) return 0;

@@ -164,6 +164,7 @@ int run_q4(ruyb200_ctx* ctx, const char* call, const ruyb200_mul_desc* desc, con
   m.x_dtype = d.rhs.dtype;
   m.dst_dtype = d.dst.dtype;
   m.scale_dtype = scales->dtype;
+  m.force_any = ctx_forces_generic(ctx);
   m.groups = group_list(groups);
   m.status = ctx_status_word(ctx);
   int kernel = RUYB200_KERNEL_NONE;
@@ -231,6 +232,7 @@ int ruyb200_mul_grouped_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, co
                           {groups->offsets, 4}};
   rc = check_pointers(ctx_device(ctx), call, list, 7);
   if (rc) return rc;
+  m.force_any = ctx_forces_generic(ctx);
   m.groups = group_list(groups);
   m.status = ctx_status_word(ctx);
   int kernel = RUYB200_KERNEL_NONE;

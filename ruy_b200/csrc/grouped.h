@@ -46,6 +46,7 @@ struct GroupedI8Mul {
   const int32_t* mfp_pc;     // per row, or nullptr
   const int32_t* mexp_pc;
   uint8_t w_dtype, x_dtype, dst_dtype, rounding_x86;
+  uint8_t force_any;         // keep the mul on the CUDA-core kernel
   GroupList groups;
   int* status;               // receives a non-zero code when a bounded wait gives up
 };
@@ -67,6 +68,7 @@ struct Q4Mul {
   const float* bias;           // per row, or nullptr
   float clamp_min, clamp_max;
   uint8_t w_signed, x_dtype, dst_dtype, scale_dtype;
+  uint8_t force_any;           // keep the mul on the CUDA-core kernel
   GroupList groups;
   int* status;
 };

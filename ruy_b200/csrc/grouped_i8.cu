@@ -748,7 +748,7 @@ bool aligned_layout(const GroupedI8Mul& m) {
 }  // namespace
 
 cudaError_t launch_grouped_i8(const GroupedI8Mul& m, int sm_count, cudaStream_t stream, int* kernel) {
-  if (!aligned_layout(m)) {
+  if (m.force_any || !aligned_layout(m)) {
     *kernel = RUYB200_KERNEL_GENERIC;
     return launch_any(m, stream);
   }

@@ -39,6 +39,7 @@ int ctx_validate(const ruyb200_mul_desc* d);
 bool ptr_on_device(const void* p);
 int ctx_rounding_is_x86(ruyb200_ctx* ctx, int rounding_mode);
 bool ctx_trace(ruyb200_ctx* ctx);
+bool ctx_forces_generic(ruyb200_ctx* ctx);   // RUYB200_FORCE_KERNEL=generic
 int ctx_run_mul_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* d);
 int ctx_plan_item(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, BatchItem* out, bool* fits,
                   std::vector<CacheKey>* pinned);

@@ -687,7 +687,7 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_q4(const Q4Mul& m, int sm_count, cudaStream_t stream, int* kernel) {
-  if (staged_layout(m)) {
+  if (!m.force_any && staged_layout(m)) {
     *kernel = RUYB200_KERNEL_Q4;
     return launch_tensor(m, sm_count, stream);
   }

@@ -768,3 +768,89 @@ def test_expert_layer_in_8_and_4_bits():
     assert torch.equal(y.double(), want())
     del graph
     context.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,rows,kernel", [
+    ([3, 0, 2], 300, "grouped_mma"), ([1] * 20, 64, "grouped_mma"), ([9, 1], 300, "grouped_tc"), ([200] * 3, 100, "grouped_tc"),
+    ([20, 300, 0, 45, 1, 64, 700, 33] * 5, 1100, "grouped_tc")], ids=["few", "singles", "some", "narrow", "pairs"])
+@pytest.mark.parametrize("lhs,rhs,dst,zps", [
+    ("i8", "i8", "i8", (0, 0, 0)), ("i8", "u8", "u8", (0, 131, 7)), ("i8", "i8", "i16", (0, -5, 100)), ("i8", "i8", "i32", (0, 3, 0)),
+    ("u8", "u8", "u8", (128, 77, 3))])
+def test_grouped_kernels_types_and_whole_words(ctx, sizes, rows, kernel, lhs, rhs, dst, zps):
+    # destinations whose columns are whole words take another way out of the tensor-core kernel than others
+    for r, dst_pad in ((rows, 0), (rows - rows % 32 + 32, 0), (rows, 4 - rows % 4 + 4), (rows, 5)):
+        I8Case(sizes, r, 144, lhs, rhs, dst, *zps, pad=2, dst_pad=dst_pad).check(ctx, kernel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponents", [(-31, -14), (-14, -1), (-1, 3), (-31, 3)])
+@pytest.mark.parametrize("dst,zp", [("i8", -128), ("u8", 255), ("i16", -32768), ("i16", 32767)])
+@pytest.mark.parametrize("sizes", [[2, 1], [50, 9]])
+def test_grouped_every_shift(ctx, exponents, dst, zp, sizes):
+    # shifts of 32 and more take a shorter way; the others, and zero points that do not fit into the rounding term, do not
+    c = I8Case(sizes, 96, 32, dst=dst, dst_zp=zp, rhs_zp=1)
+    r = np.random.default_rng(7)
+    c.mexp = r.integers(exponents[0], exponents[1], c.mexp.shape).astype(np.int32)
+    c.mfp = r.integers(2 ** 20, 2 ** 24, c.mfp.shape).astype(np.int32)      # results stay within 32 bits at every shift
+    c.check(ctx)
+
+
+@pytest.mark.gpu
+def test_forced_generic_kernel(monkeypatch):
+    import torch
+    monkeypatch.setenv("RUYB200_FORCE_KERNEL", "generic")
+    c = rb.Context(0, torch.cuda.default_stream().cuda_stream or 1)
+    I8Case([40, 0, 9, 300], 96, 160, rhs_zp=3, dst_zp=-4).check(c, "generic")
+    Q4Case(70, 320, sizes=[3, 0, 20], x="bf16", block=32, zeros=True).check(c, "generic")
+    Q4Case(70, 320, 4, block=128, whole=False).check(c, "generic")
+    c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[1] * 30, [17, 0, 41, 90, 1]])
+@pytest.mark.parametrize("x,block", [("f32", 32), ("f16", 64), ("bf16", 128), ("f32", 256)])
+def test_grouped_q4_many_rows_and_long_groups(ctx, sizes, x, block):
+    Q4Case(700, 1056, sizes=sizes, x=x, block=block, zeros=True, pad=1).check(ctx, "q4")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,power", [("f16", -20), ("f16", 8), ("bf16", -100), ("bf16", 100), ("f32", -100), ("f32", 100)])
+def test_q4_small_and_large_activations(ctx, x, power):
+    import torch
+    c = Q4Case(60, 640, 5, x=x, y="f32", block=64, zeros=True, bias=False)
+    c.values = (c.values.double() * 2.0 ** power).to(c.T[x])
+    c.x[:, :c.depth] = c.values
+    c.check(ctx, "q4")      # sums of small integers times a power of two: exact
+
+
+@pytest.mark.gpu
+def test_q4_every_weight_and_zero_point(ctx):
+    """Every (q, z) that the documentation allows, one at a time, against its exact value."""
+    import torch
+    for signed in (True, False):
+        low = -8 if signed else 0
+        for x in ("f32", "f16", "bf16"):
+            c = Q4Case(16, 32, 32, x=x, y="f32", block=32, signed=signed, zeros=True, bias=False)
+            w = torch.zeros((16, 32), dtype=torch.uint8)
+            for k in range(32):
+                w[:, k] = k % 16
+            c.w = (w[:, 0::2] | (w[:, 1::2] << 4)).reshape(1, 16, 16)
+            c.zeros = torch.arange(low, low + 16).to(torch.int8).reshape(1, 16, 1)
+            c.scales = torch.ones((1, 16, 1))
+            c.values = torch.eye(32).to(c.T[x])
+            c.x[:, :32] = c.values
+            got = c.logical(c.run(ctx)).double()            # [k][z]
+            q = torch.arange(32) % 16
+            q = torch.where(q > 7, q - 16, q) if signed else q
+            assert torch.equal(got, (q[:, None] - torch.arange(low, low + 16)[None, :]).double())
+
+
+@pytest.mark.gpu
+def test_same_result_every_time(ctx):
+    import torch
+    c = Q4Case(520, 4096, 5, x="f32", whole=False, block=128)
+    t = c.tensors()
+    first = c.run(ctx, t).clone()
+    for _ in range(5):
+        assert torch.equal(c.run(ctx, t), first)
