@@ -661,10 +661,12 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
     if (a.block_steps == 1 << i) a.block_shift = i;
   }
   const int pieces = m.x_dtype == RUYB200_F32 ? 3 : 1;
-  long long expected = m.cols;
-  if (m.groups.offsets) expected = min((long long)m.cols, 2 * ((m.cols + (long long)m.groups.count - 1) / m.groups.count));
-  // columns per pass, a whole number of MMA tiles: up to 16 fp32 or 32 half ones (6 and 4 tiles)
-  const bool few = expected * pieces <= 16;
+  // Columns per pass, a whole number of MMA tiles: 16 half or 5 fp32 ones (two tiles), or 32 and 16 (four and six), whose
+  // warps hold more sums and so hide less of each other's latency.  A group of about 12 columns or fewer is better served
+  // by several narrow passes side by side (16 groups x 2048 x 2048, 131 columns: bf16 26 us against 36, fp32 45 against 50),
+  // one of 32 by wide passes (8 x 1024 x 1024, 256 fp32 columns: 34 us against 50).
+  const long long share = m.groups.offsets ? (m.cols + (long long)m.groups.count - 1) / m.groups.count : m.cols;
+  const bool few = m.groups.offsets ? share <= 12 : share * pieces <= 16;
   a.room = few ? 16 / pieces : (pieces == 3 ? 16 : 32);
   const int esz = pieces == 3 ? 4 : 2;
   a.x_vec = m.x_stride_k == 1 && (((uintptr_t)m.x | (uintptr_t)(m.x_stride_c * esz)) & 15) == 0;
@@ -677,7 +679,7 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
   a.slabs_per = (slabs + a.split - 1) / a.split;
   // the largest segment: its rows, and the padding between them
   const int slab_columns = pieces == 3 ? Carried<kFloat3>::kSlabColumns : Carried<kBf16>::kSlabColumns;
-  a.pass_lanes = (int)min(4ll, (m.cols + (long long)a.room - 1) / a.room);
+  a.pass_lanes = (int)min(8ll, (m.cols + (long long)a.room - 1) / a.room);
   a.x_bytes = pieces * (slab_columns * kSlab * 2 + a.room * 64);
   if (pieces == 3) return few ? launch_by_block<kFloat3, 2>(a, stream) : launch_by_block<kFloat3, 6>(a, stream);
   if (m.x_dtype == RUYB200_F16) return few ? launch_by_block<kHalf, 2>(a, stream) : launch_by_block<kHalf, 4>(a, stream);
