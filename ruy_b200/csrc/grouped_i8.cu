@@ -248,24 +248,39 @@ struct TcGroupedArgs {
   int32_t dst_words;    // 8-bit destinations: four rows of a column are an aligned word
 };
 
+// The four MMAs of 32 bytes of depth that a stage holds.  The issuing thread is alone and the tensor core's queue is short,
+// so what it executes between two MMAs counts: the descriptors advance by one addition each.  `accumulate` is false for the
+// first stage of a tile.
 template <bool kPair>
-__device__ __forceinline__ void tc_mma_i8(uint32_t tmem, uint32_t desc_a, uint32_t desc_b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_stage(uint32_t tmem, uint32_t desc_a, uint32_t desc_b, uint32_t idesc, bool accumulate) {
   // 128-byte swizzled, depth-contiguous tiles: rows 128 bytes apart, groups of 8 rows 1024 bytes apart
   constexpr uint32_t kHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
   if (kPair) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.u32 p, %4, 0;\n\t"
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 t, 0, 0;\n\t"
         "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, p;\n\t"
+        "add.u32 la, %1, 2;\n\tadd.u32 lb, %2, 2;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, t;\n\t"
+        "add.u32 la, %1, 4;\n\tadd.u32 lb, %2, 4;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, t;\n\t"
+        "add.u32 la, %1, 6;\n\tadd.u32 lb, %2, 6;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, t;\n\t}"
         ::"r"(tmem), "r"(desc_a), "r"(desc_b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kHigh)
         : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.u32 p, %4, 0;\n\t"
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 t, 0, 0;\n\t"
         "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t"
+        "add.u32 la, %1, 2;\n\tadd.u32 lb, %2, 2;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, t;\n\t"
+        "add.u32 la, %1, 4;\n\tadd.u32 lb, %2, 4;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, t;\n\t"
+        "add.u32 la, %1, 6;\n\tadd.u32 lb, %2, 6;\n\tmov.b64 da, {la, %5};\n\tmov.b64 db, {lb, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, t;\n\t}"
         ::"r"(tmem), "r"(desc_a), "r"(desc_b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kHigh)
         : "memory");
   }
@@ -503,19 +518,17 @@ grouped_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       ok = __all_sync(0xffffffffu, mbarrier_wait(&acc_empty[buf], ((count >> 1) & 1) ^ 1, abortp));
       tc_after_sync();
       const uint32_t acc = tmem + buf * kTcAccCols;
+      const uint32_t idesc = a.idesc | tc_width(width), idesc_sums = a.idesc | tc_width(S::kStep);
       for (int kb = 0; kb < a.k_blocks && ok; kb++) {
-        ok = __all_sync(0xffffffffu, mbarrier_wait(&full[s], ph, abortp));
+        if (!mbarrier_try(&full[s], ph)) ok = mbarrier_wait(&full[s], ph, abortp);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_after_sync();
         const uint32_t dw = desc0 + s * (S::kStageBytes >> 4), dx = dw + (kTcWBytes >> 4);
         if (tc_elect()) {
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const bool more = (kb | k) != 0;
-            tc_mma_i8<kPair>(acc, dw + 2 * k, dx + 2 * k, a.idesc | tc_width(width), more);
-            if (a.row_sums) tc_mma_i8<kPair>(acc + S::kSumCol, dw + 2 * k, desc_ones + 2 * k, a.idesc | tc_width(S::kStep), more);
-            if (!kPair && a.token_sums) tc_mma_i8<kPair>(acc + kTcTokenCol, desc_ones + 2 * k, dx + 2 * k, a.idesc | tc_width(width), more);
-          }
+          tc_mma_stage<kPair>(acc, dw, dx, idesc, kb != 0);
+          if (a.row_sums) tc_mma_stage<kPair>(acc + S::kSumCol, dw, desc_ones, idesc_sums, kb != 0);
+          if (!kPair && a.token_sums) tc_mma_stage<kPair>(acc + kTcTokenCol, desc_ones, dx, idesc, kb != 0);
           tc_commit<kPair>(&empty[s]);
           if (kb == a.k_blocks - 1) tc_commit<kPair>(&acc_full[buf]);
         }
