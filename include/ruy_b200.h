@@ -296,7 +296,7 @@ RUYB200_API int ruyb200_mul_grouped_async(ruyb200_ctx* ctx, const ruyb200_mul_de
  * elements and even, zero_point 0.  desc->rhs: RUYB200_F32, F16 or BF16, any order and stride.  desc->dst: F32 or the
  * type of rhs, any order and stride.  desc->params: accum_dtype RUYB200_F32, bias float[rows] or NULL, clamp_* in .f; NaN
  * results stay NaN whatever the clamp.  Sums are held in 32 bits; they may be formed over (part of) a block before its
- * scale is applied.  Weights whose base address is a multiple of 16
+ * scale is applied; of fp32 activations below 2^-112 the lowest bits may be lost.  Weights whose base address is a multiple of 16
  * bytes and whose stride is one of 32 elements (lhs_stride also of the row stride) run on the tensor cores, anything
  * else on a slower CUDA-core kernel. */
 RUYB200_API int ruyb200_mul_q4_async(ruyb200_ctx* ctx, const ruyb200_mul_desc* desc, const ruyb200_q4_scales* scales);

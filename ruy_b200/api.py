@@ -361,8 +361,10 @@ class Q4Matrix:
 
     def _fields(self):
         lay = self.layout
-        return (_ptr_and_dtype(self.data)[0] or 0, lay.rows, lay.cols, lay.stride, 0, lay.order, _abi.I4 if self.signed else _abi.U4,
-                0, 0)
+        ptr, dt = _ptr_and_dtype(self.data)
+        if dt not in (None, _abi.I8, _abi.U8):
+            raise TypeError("Q4Matrix.data must be uint8 or int8 (two elements to a byte)")
+        return ptr or 0, lay.rows, lay.cols, lay.stride, 0, lay.order, _abi.I4 if self.signed else _abi.U4, 0, 0
 
     def to_desc(self):
         return _abi.MatrixDesc(*self._fields())

@@ -66,7 +66,8 @@ cudaError_t launch_any(const GroupedI8Mul& m, cudaStream_t stream) {
 // Bound by the weights' bytes.  A CTA owns 16 weight rows of a group and its warps split the depth; every weight byte is
 // loaded once per 8 columns, straight into MMA fragments (m16n8k32): the depth may be taken in any order as long as
 // both operands take the same, so a lane's 16 consecutive bytes are its share of two MMAs.  Sums for the zero points come
-// from the same registers.  CTAs of empty groups leave at once.
+// from the same registers.  CTAs of empty groups leave at once.  Measured: two columns in two of eight groups of 4096 x 4096,
+// 33.6 MB of weights, 10.9 us (3.1 TB/s over all; launch, offsets and the first loads' latency are about half of it).
 constexpr int kMmaWarps = 4;
 
 template <bool kWSigned, bool kXSigned>
@@ -218,6 +219,9 @@ cudaError_t launch_mma(const GroupedI8Mul& m, cudaStream_t stream) {
 // against ones; the sums of the tokens (needed for one of the weights) are one more MMA of ones against the tokens, whose
 // every row then holds them: each lane finds what it needs in its own row of tensor memory, and no pass over the operands
 // and no workspace is needed.  Tiles are narrower then, to leave room in tensor memory.
+//
+// Measured: 8 x 4096 x 4096, 8192 columns 124.7 us (2.2 POP/s; 9 rounds of tiles where 8.4 are needed, tiles of 205 columns on
+// average, about 10 us of epilogue that the next tile does not hide); 64 x 1024 x 2048, 512 columns 32.6 us (4.2 TB/s).
 constexpr int kTileM = 128;
 constexpr int kTileK = 128;                 // bytes of depth per stage
 constexpr int kTcWBytes = kTileM * kTileK;

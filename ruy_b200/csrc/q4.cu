@@ -105,6 +105,11 @@ cudaError_t launch_any(const Q4Mul& m, cudaStream_t stream) {
 // are on their way in registers.  The scales of a slab are fetched two slabs ahead, one row per two lanes, and handed to
 // the lanes that need them by shuffles.
 //
+// Measured on one B200: 16384 x 16384, one f16 column 47.6 us (138.5 MB at 2.9 TB/s); 4096 x 16384, 16 bf16 columns 25.3 us;
+// 4096 x 4096, one bf16 column 8.9 us, of which 6 are launch, set-up and the two cluster barriers.  The large one is bound by
+// instruction issue and the ALU pipe (45 instructions per 16 rows x 32 deep, 25 of them the arithmetic above): the same
+// kernel without its arithmetic takes 28 us.
+//
 // Fragments.  The MMAs may take the depth in any order as long as both operands take the same.  Lane t of a quad owns
 // 8 consecutive depth positions of every 32 (a step): one 32-bit word of weights holds its share for two MMAs, and masks
 // pick out the pairs (0,4), (1,5), (2,6), (3,7) that end up in the halves of a register.  The activations are stored in
@@ -143,12 +148,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], bool fresh, uint32_t a0
   const float z0 = fresh ? 0.f : c[0], z1 = fresh ? 0.f : c[1], z2 = fresh ? 0.f : c[2], z3 = fresh ? 0.f : c[3];
   if (kType == kHalf) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   } else {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   }
 }
 
@@ -238,6 +243,7 @@ __device__ __forceinline__ void load_x8(const Q4Args& a, int col, int k, X8<kTyp
 
 // The upper 16 bits of a float are a bf16 that differs from it by less than one step, so what is left after taking them
 // away is exact, and three times 8 bits are all of the significand's 24.  Infinities and NaN live in the first piece alone.
+// The smallest bf16 is 2**-133: of activations below about 2**-112 the lowest bits are lost, at most 2**-133 each.
 __device__ __forceinline__ void split3(uint32_t bits, uint32_t (&piece)[3]) {
   const float x = __uint_as_float(bits);
   const uint32_t h = bits & 0xffff0000u;
@@ -642,7 +648,7 @@ cudaError_t launch_by_block(const Q4Args& a, cudaStream_t stream) {
 
 // The copy engine's needs: 16-byte aligned rows, groups a whole number of rows apart; indices of 32 bits.
 bool staged_layout(const Q4Mul& m) {
-  if (m.depth == 0 || m.depth > (1 << 30) || m.rows > (1 << 30) || ((uintptr_t)m.w & 15) != 0 || m.w_stride % 32 != 0) return false;
+  if (m.depth == 0 || m.depth > (1 << 30) || m.rows > (1 << 30) || m.cols > (1 << 30) || ((uintptr_t)m.w & 15) != 0 || m.w_stride % 32 != 0) return false;
   if (m.groups.lhs_stride % m.w_stride != 0) return false;
   const int64_t per = m.groups.lhs_stride / m.w_stride;
   if (per > 0x7fffffff) return false;

@@ -191,6 +191,8 @@ def test_new_argument_classes_check_their_types():
         rb.Groups(np.zeros(3, np.int16), 0).to_desc()
     with pytest.raises(TypeError):
         rb.Q4Scales(np.zeros(4, np.float32), 32, 1, np.zeros(4, np.uint8)).to_desc()
+    with pytest.raises(TypeError):
+        rb.Q4Matrix(np.zeros(4, np.float32), rb.Layout(1, 8, 8, RowMajor), None).to_desc()
 
 
 # ---- on a GPU -------------------------------------------------------------------------------------------
