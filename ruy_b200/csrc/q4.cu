@@ -531,6 +531,11 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Only meets: for reads that have returned their values.
+__device__ __forceinline__ void cluster_barrier_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ float load_of_rank(const float* p, uint32_t rank) {
   uint32_t at;
   float v;
@@ -598,9 +603,13 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
       }
       if (row0 + r < a.m.rows) store_q4(a.m, g, row0 + r, c0 + c, v * kUnit<kType>);
     }
-    asm volatile("fence.proxy.async;" ::: "memory");            // the copy engine writes where `part` was
-    if (a.split > 1) cluster_barrier(); else __syncthreads();   // `part` may be overwritten, or its CTA gone
-    asm volatile("fence.proxy.async;" ::: "memory");
+    // `part` may be overwritten by the copy engine, or its CTA be gone, once everybody has read it.  Neither needs this pass's
+    // stores to have arrived anywhere, and waiting for them would cost microseconds, so the barrier orders nothing.
+    const bool more = c0 + (int)gridDim.z * a.room < end;
+    if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (a.split > 1) cluster_barrier_relaxed();
+    else if (more) __syncthreads();
+    if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (abort_flag && threadIdx.x == 0) {
     // give copies in flight a bounded chance to land before the CTA exits: every stage that was filled and not waited for
