@@ -105,8 +105,8 @@ cudaError_t launch_any(const Q4Mul& m, cudaStream_t stream) {
 // are on their way in registers.  The scales of a slab are fetched two slabs ahead, one row per two lanes, and handed to
 // the lanes that need them by shuffles.
 //
-// Measured on one B200: 16384 x 16384, one f16 column 47.6 us (138.5 MB at 2.9 TB/s); 4096 x 16384, 16 bf16 columns 25.3 us;
-// 4096 x 4096, one bf16 column 8.9 us, of which 6 are launch, set-up and the two cluster barriers.  The large one is bound by
+// Measured on one B200: 16384 x 16384, one f16 column 47.6 us (138.5 MB at 2.9 TB/s); 4096 x 16384, 16 bf16 columns 24.9 us;
+// 4096 x 4096, one bf16 column 8.5 us, of which 6 are launch, set-up and the cluster's barriers.  The large one is bound by
 // instruction issue and the ALU pipe (45 instructions per 16 rows x 32 deep, 25 of them the arithmetic above): the same
 // kernel without its arithmetic takes 28 us.
 //
