@@ -686,7 +686,10 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
   const int esz = pieces == 3 ? 4 : 2;
   a.x_vec = m.x_stride_k == 1 && (((uintptr_t)m.x | (uintptr_t)(m.x_stride_c * esz)) & 15) == 0;
   const long long active = m.groups.offsets ? min((long long)m.groups.count, (long long)m.cols) : 1;
-  const long long row_tiles = ((long long)m.rows + kRows - 1) / kRows * active;
+  // CTAs side by side for the passes that a group of four times the mean share would take (a CTA without a pass still has to
+  // start: 45 groups x 2396 x 363, 120 columns: 40 us with eight each, 28 with one)
+  a.pass_lanes = (int)min(8ll, (min((long long)m.cols, m.groups.offsets ? 4 * share : share) + a.room - 1) / a.room);
+  const long long row_tiles = ((long long)m.rows + kRows - 1) / kRows * active * ((share + a.room - 1) / a.room);
   const int slabs = (int)(((long long)m.depth + kSlab - 1) / kSlab);
   // as many CTAs per cluster as still let all run at once, two per SM
   const int split = (int)max(1ll, min(min((long long)kMaxSplit, (long long)slabs), 2 * sm_count / row_tiles));
@@ -694,7 +697,6 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
   a.slabs_per = (slabs + a.split - 1) / a.split;
   // the largest segment: its rows, and the padding between them
   const int slab_columns = pieces == 3 ? Carried<kFloat3>::kSlabColumns : Carried<kBf16>::kSlabColumns;
-  a.pass_lanes = (int)min(8ll, (m.cols + (long long)a.room - 1) / a.room);
   a.x_bytes = pieces * (slab_columns * kSlab * 2 + a.room * 64);
   if (pieces == 3) return few ? launch_by_block<kFloat3, 2>(a, stream) : launch_by_block<kFloat3, 6>(a, stream);
   if (m.x_dtype == RUYB200_F16) return few ? launch_by_block<kHalf, 2>(a, stream) : launch_by_block<kHalf, 4>(a, stream);
