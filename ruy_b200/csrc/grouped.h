@@ -32,6 +32,44 @@ __device__ __forceinline__ void group_columns(const GroupList& groups, int g, in
   *end = max(e, b);
 }
 
+// A grid's second axis has a slot for every group, or, where tokens are far fewer than groups, for every group that can have
+// a column: CTAs of empty groups cost their start (60 groups x 3728 x 597 of 4 bits, 4 columns: 14.0 us with all, 9.7 with 4).
+// In the second form slot n stands for the n-th group that has columns, found by a scan of the offsets, which costs about
+// 1 us and is not worth it for half as many tokens as groups (64 x 1024 x 2048, 32 columns: 18.4 us against 16.8).
+//
+// The group of a slot; false when it has none, or an empty one.  A whole warp calls it.  More groups than slots have columns
+// only when offsets decrease; callers go on to slot + gridDim.y.
+__device__ __forceinline__ bool nth_group(const GroupList& groups, int cols, int slot, int* g, int* begin, int* end) {
+  if (gridDim.y == (unsigned)groups.count) {
+    if (slot >= groups.count) return false;
+    *g = slot;
+    group_columns(groups, slot, cols, begin, end);
+    return *end > *begin;
+  }
+  const int lane = threadIdx.x & 31;
+  if (slot >= groups.count) return false;
+  int seen = 0;
+  for (int g0 = 0; g0 < groups.count; g0 += 32) {
+    int b = 0, e = 0;
+    if (g0 + lane < groups.count) group_columns(groups, g0 + lane, cols, &b, &e);
+    const uint32_t there = __ballot_sync(0xffffffffu, e > b);
+    const int n = __popc(there);
+    if (slot < seen + n) {
+      const int at = __fns(there, 0, slot - seen + 1);
+      *g = g0 + at;
+      *begin = __shfl_sync(0xffffffffu, b, at);
+      *end = __shfl_sync(0xffffffffu, e, at);
+      return true;
+    }
+    seen += n;
+  }
+  return false;
+}
+// Slots of a launch.
+inline unsigned group_slots(const GroupList& groups, int cols) {
+  return (unsigned)(groups.offsets && groups.count / 4 >= cols ? cols : groups.count);
+}
+
 // A grouped 8-bit mul.  Element (r, k) of group g's weights is w[g * lhs_stride + r * w_stride + k], element (k, c) of the
 // activations x[c * x_stride + k], element (r, c) of the destination dst[c * dst_stride + r].
 struct GroupedI8Mul {

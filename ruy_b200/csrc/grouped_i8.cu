@@ -66,8 +66,8 @@ cudaError_t launch_any(const GroupedI8Mul& m, cudaStream_t stream) {
 // Bound by the weights' bytes.  A CTA owns 16 weight rows of a group and its warps split the depth; every weight byte is
 // loaded once per 8 columns, straight into MMA fragments (m16n8k32): the depth may be taken in any order as long as
 // both operands take the same, so a lane's 16 consecutive bytes are its share of two MMAs.  Sums for the zero points come
-// from the same registers.  CTAs of empty groups leave at once.  Measured: two columns in two of eight groups of 4096 x 4096,
-// 33.6 MB of weights, 10.9 us (3.1 TB/s over all; launch, offsets and the first loads' latency are about half of it).
+// from the same registers.  Measured: two columns in two of eight groups of 4096 x 4096,
+// 33.6 MB of weights, 10.9 us, of which launch, offsets and the first loads' latency are about half.
 constexpr int kMmaWarps = 4;
 
 template <bool kWSigned, bool kXSigned>
@@ -107,16 +107,14 @@ template <bool kWSigned, bool kXSigned>
 __global__ void __launch_bounds__(32 * kMmaWarps) grouped_i8_mma_kernel(const __grid_constant__ GroupedI8Mul m) {
   constexpr int kPart = 7;   // per lane: 4 sums, an activation sum, 2 weight sums
   __shared__ int32_t part[kMmaWarps - 1][kPart][32];
-  const int g = blockIdx.y;
-  int begin, end;
-  group_columns(m.groups, g, m.cols, &begin, &end);
-  if (begin == end) return;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, quad = lane >> 2, t = lane & 3;
   const int r0 = blockIdx.x * 16 + quad, r1 = r0 + 8;
-  const uint8_t* const base = (const uint8_t*)m.w + (int64_t)g * m.groups.lhs_stride;
+  const bool need_w = m.zp_x != 0, need_x = m.zp_w != 0;
+  int g, begin, end;
+  for (int slot = blockIdx.y; nth_group(m.groups, m.cols, slot, &g, &begin, &end); slot += gridDim.y) {
+    const uint8_t* const base = (const uint8_t*)m.w + (int64_t)g * m.groups.lhs_stride;
   const uint8_t* const row0 = base + (int64_t)min(r0, m.rows - 1) * m.w_stride;
   const uint8_t* const row1 = base + (int64_t)min(r1, m.rows - 1) * m.w_stride;
-  const bool need_w = m.zp_x != 0, need_x = m.zp_w != 0;
   for (int c0 = begin; c0 < end; c0 += 8) {
     int32_t acc[4] = {}, xsum = 0, wsum0 = 0, wsum1 = 0;
     // columns past the group's last repeat it; their sums are not stored
@@ -190,10 +188,11 @@ __global__ void __launch_bounds__(32 * kMmaWarps) grouped_i8_mma_kernel(const __
     }
     __syncthreads();   // `part` may be written again
   }
+  }
 }
 
 cudaError_t launch_mma(const GroupedI8Mul& m, cudaStream_t stream) {
-  const dim3 grid((unsigned)((m.rows + 15) / 16), m.groups.count);
+  const dim3 grid((unsigned)((m.rows + 15) / 16), group_slots(m.groups, m.cols));
   const bool ws = m.w_dtype == RUYB200_I8, xs = m.x_dtype == RUYB200_I8;
   if (ws && xs) grouped_i8_mma_kernel<true, true><<<grid, 32 * kMmaWarps, 0, stream>>>(m);
   else if (ws) grouped_i8_mma_kernel<true, false><<<grid, 32 * kMmaWarps, 0, stream>>>(m);

@@ -551,10 +551,8 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kStages<kType>], empty[kStages<kType>];
   __shared__ int abort_flag;
-  const int g = blockIdx.y;
-  int begin, end;
-  group_columns(a.m.groups, g, a.m.cols, &begin, &end);
-  if (begin == end) return;   // the whole cluster belongs to the group
+  int slot = blockIdx.y, g, begin, end;
+  if (!nth_group(a.m.groups, a.m.cols, slot, &g, &begin, &end)) return;   // the whole cluster has the same slot
   uint8_t* const data = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   float* const part = reinterpret_cast<float*>(data);   // between two passes, when the ring is empty
   uint8_t* const xs = data + kStages<kType> * kStageBytes;
@@ -574,7 +572,9 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
   const int slabs = (a.m.depth + kSlab - 1) / kSlab;
   const int slab0 = min(rank * a.slabs_per, slabs), slab1 = min(slab0 + a.slabs_per, slabs);
   volatile int* abortp = &abort_flag;
-  Ring ring = {full, empty, data, &map, (int)(g * a.group_rows + row0), 0, 0, 0, 0, true};
+  Ring ring = {full, empty, data, &map, 0, 0, 0, 0, 0, true};
+  for (;;) {
+  ring.row = (int)(g * a.group_rows + row0);
   // a long group's passes are shared out along the grid's third axis
   for (int c0 = begin + (int)blockIdx.z * a.room; c0 < end; c0 += (int)gridDim.z * a.room) {
     const int n = min(a.room, end - c0);
@@ -611,6 +611,12 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
     else if (more) __syncthreads();
     if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  slot += gridDim.y;
+  if (!nth_group(a.m.groups, a.m.cols, slot, &g, &begin, &end)) break;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // as between two passes
+  __syncthreads();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
   if (abort_flag && threadIdx.x == 0) {
     // give copies in flight a bounded chance to land before the CTA exits: every stage that was filled and not waited for
     for (int s = 0; s < kStages<kType>; s++) {
@@ -634,7 +640,7 @@ cudaError_t launch_staged(const Q4Args& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(((long long)m.rows + kRows - 1) / kRows * a.split), m.groups.count, a.pass_lanes);
+  cfg.gridDim = dim3((unsigned)(((long long)m.rows + kRows - 1) / kRows * a.split), group_slots(m.groups, m.cols), a.pass_lanes);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -856,3 +856,38 @@ def test_same_result_every_time(ctx):
     first = c.run(ctx, t).clone()
     for _ in range(5):
         assert torch.equal(c.run(ctx, t), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets,cols", [([0, 1, 0, 1, 0, 2], 2), ([3, 0, 3, 1, 3, 2, 3], 3), ([0, 1] * 40 + [4], 4)])
+def test_more_groups_with_columns_than_columns(ctx, offsets, cols):
+    """Offsets that decrease can give every column to many groups; with one matrix of weights for all, the answer is plain."""
+    import torch
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    for rows, depth in ((40, 64), (200, 600)):
+        c = I8Case([cols], rows, depth, rhs_zp=2)
+        t = c.tensors()
+        lhs, rhs, p, dst, groups = c.args(t)
+        rb.mul_grouped_async(lhs, rhs, p, ctx, dst, rb.Groups(off, 0))
+        ctx.sync()
+        np.testing.assert_array_equal(t["y"].cpu().numpy(), c.want())
+        q = Q4Case(rows, depth, sizes=[cols], x="bf16", block=32, zeros=True, shared=True)
+        q.offsets = off.cpu()
+        t = q.tensors()
+        got = q.logical(q.run(ctx, t)).double()
+        q.offsets = torch.tensor([0, cols], dtype=torch.int32)
+        assert torch.equal(got, q.want()[0].to(torch.bfloat16).double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [33, 200, 1024])
+def test_few_tokens_over_many_groups(ctx, groups):
+    r = np.random.default_rng(groups)
+    sizes = [0] * groups
+    for g in r.integers(0, groups, 5):
+        sizes[g] += 1
+    sizes[-1] += 1
+    I8Case(sizes, 70, 96, pad=2, first=1, rhs_zp=1).check(ctx, "grouped_mma")
+    Q4Case(70, 96, sizes=sizes, x="f16", block=32, zeros=True, pad=2, first=1).check(ctx, "q4")
+    sizes[3] += 900
+    I8Case(sizes, 70, 96, pad=2, first=1, rhs_zp=1).check(ctx)
