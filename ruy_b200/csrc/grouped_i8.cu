@@ -113,81 +113,81 @@ __global__ void __launch_bounds__(32 * kMmaWarps) grouped_i8_mma_kernel(const __
   int g, begin, end;
   for (int slot = blockIdx.y; nth_group(m.groups, m.cols, slot, &g, &begin, &end); slot += gridDim.y) {
     const uint8_t* const base = (const uint8_t*)m.w + (int64_t)g * m.groups.lhs_stride;
-  const uint8_t* const row0 = base + (int64_t)min(r0, m.rows - 1) * m.w_stride;
-  const uint8_t* const row1 = base + (int64_t)min(r1, m.rows - 1) * m.w_stride;
-  for (int c0 = begin; c0 < end; c0 += 8) {
-    int32_t acc[4] = {}, xsum = 0, wsum0 = 0, wsum1 = 0;
-    // columns past the group's last repeat it; their sums are not stored
-    const uint8_t* const xrow = (const uint8_t*)m.x + (int64_t)min(c0 + quad, end - 1) * m.x_stride;
-    // a step is 256 bytes of every row: 4 pieces of 16 per lane, all loads before the first use
-    for (int k0 = warp * 256; k0 < m.depth; k0 += 256 * kMmaWarps) {
-      uint4 a[4], b[4], x[4];
+    const uint8_t* const row0 = base + (int64_t)min(r0, m.rows - 1) * m.w_stride;
+    const uint8_t* const row1 = base + (int64_t)min(r1, m.rows - 1) * m.w_stride;
+    for (int c0 = begin; c0 < end; c0 += 8) {
+      int32_t acc[4] = {}, xsum = 0, wsum0 = 0, wsum1 = 0;
+      // columns past the group's last repeat it; their sums are not stored
+      const uint8_t* const xrow = (const uint8_t*)m.x + (int64_t)min(c0 + quad, end - 1) * m.x_stride;
+      // a step is 256 bytes of every row: 4 pieces of 16 per lane, all loads before the first use
+      for (int k0 = warp * 256; k0 < m.depth; k0 += 256 * kMmaWarps) {
+        uint4 a[4], b[4], x[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        a[i] = load_piece(row0, k0 + 64 * i + 16 * t, m.depth, true);
-        b[i] = load_piece(row1, k0 + 64 * i + 16 * t, m.depth, true);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = load_piece(xrow, k0 + 64 * i + 16 * t, m.depth, false);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        mma_16832<kWSigned, kXSigned>(acc, a[i].x, b[i].x, a[i].y, b[i].y, x[i].x, x[i].y);
-        mma_16832<kWSigned, kXSigned>(acc, a[i].z, b[i].z, a[i].w, b[i].w, x[i].z, x[i].w);
-        if (need_x) xsum = add16<kXSigned>(x[i], xsum);
-        if (need_w) {
-          wsum0 = add16<kWSigned>(a[i], wsum0);
-          wsum1 = add16<kWSigned>(b[i], wsum1);
+        for (int i = 0; i < 4; i++) {
+          a[i] = load_piece(row0, k0 + 64 * i + 16 * t, m.depth, true);
+          b[i] = load_piece(row1, k0 + 64 * i + 16 * t, m.depth, true);
         }
-      }
-    }
-    if (warp > 0) {
-      int32_t(*const p)[32] = part[warp - 1];
 #pragma unroll
-      for (int e = 0; e < 4; e++) p[e][lane] = acc[e];
-      p[4][lane] = xsum;
-      p[5][lane] = wsum0;
-      p[6][lane] = wsum1;
-    }
-    __syncthreads();
-    if (warp == 0) {
+        for (int i = 0; i < 4; i++) x[i] = load_piece(xrow, k0 + 64 * i + 16 * t, m.depth, false);
 #pragma unroll
-      for (int w = 0; w < kMmaWarps - 1; w++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[e] += part[w][e][lane];
-        xsum += part[w][4][lane];
-        wsum0 += part[w][5][lane];
-        wsum1 += part[w][6][lane];
-      }
-      // the lanes of a quad hold the quarters of each step
-#pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        xsum += __shfl_xor_sync(0xffffffffu, xsum, d);
-        wsum0 += __shfl_xor_sync(0xffffffffu, wsum0, d);
-        wsum1 += __shfl_xor_sync(0xffffffffu, wsum1, d);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int r = h ? r1 : r0;
-        const bool there = r < m.rows;
-        const int64_t ch = (int64_t)g * m.groups.channel_stride + r;
-        const int32_t bias = there && m.bias ? m.bias[ch] : 0;
-        const int32_t mfp = there && m.mfp_pc ? m.mfp_pc[ch] : m.mfp;
-        const int32_t mexp = there && m.mexp_pc ? m.mexp_pc[ch] : m.mexp;
-        const uint32_t row_term = (uint32_t)bias - (uint32_t)m.zp_x * (uint32_t)(h ? wsum1 : wsum0) +
-                                  (uint32_t)m.zp_x * (uint32_t)m.zp_w * (uint32_t)m.depth;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int c = c0 + 2 * t + e;
-          const int32_t xs = __shfl_sync(0xffffffffu, xsum, (2 * t + e) * 4);   // the quad that summed this column
-          if (there && c < end) {
-            store_grouped(m, r, c,
-                          finish_grouped((int32_t)((uint32_t)acc[2 * h + e] - (uint32_t)m.zp_w * (uint32_t)xs), (int32_t)row_term, mfp, mexp, m));
+        for (int i = 0; i < 4; i++) {
+          mma_16832<kWSigned, kXSigned>(acc, a[i].x, b[i].x, a[i].y, b[i].y, x[i].x, x[i].y);
+          mma_16832<kWSigned, kXSigned>(acc, a[i].z, b[i].z, a[i].w, b[i].w, x[i].z, x[i].w);
+          if (need_x) xsum = add16<kXSigned>(x[i], xsum);
+          if (need_w) {
+            wsum0 = add16<kWSigned>(a[i], wsum0);
+            wsum1 = add16<kWSigned>(b[i], wsum1);
           }
         }
       }
+      if (warp > 0) {
+        int32_t(*const p)[32] = part[warp - 1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e][lane] = acc[e];
+        p[4][lane] = xsum;
+        p[5][lane] = wsum0;
+        p[6][lane] = wsum1;
+      }
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 0; w < kMmaWarps - 1; w++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[e] += part[w][e][lane];
+          xsum += part[w][4][lane];
+          wsum0 += part[w][5][lane];
+          wsum1 += part[w][6][lane];
+        }
+        // the lanes of a quad hold the quarters of each step
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) {
+          xsum += __shfl_xor_sync(0xffffffffu, xsum, d);
+          wsum0 += __shfl_xor_sync(0xffffffffu, wsum0, d);
+          wsum1 += __shfl_xor_sync(0xffffffffu, wsum1, d);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int r = h ? r1 : r0;
+          const bool there = r < m.rows;
+          const int64_t ch = (int64_t)g * m.groups.channel_stride + r;
+          const int32_t bias = there && m.bias ? m.bias[ch] : 0;
+          const int32_t mfp = there && m.mfp_pc ? m.mfp_pc[ch] : m.mfp;
+          const int32_t mexp = there && m.mexp_pc ? m.mexp_pc[ch] : m.mexp;
+          const uint32_t row_term = (uint32_t)bias - (uint32_t)m.zp_x * (uint32_t)(h ? wsum1 : wsum0) +
+                                    (uint32_t)m.zp_x * (uint32_t)m.zp_w * (uint32_t)m.depth;
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int c = c0 + 2 * t + e;
+            const int32_t xs = __shfl_sync(0xffffffffu, xsum, (2 * t + e) * 4);   // the quad that summed this column
+            if (there && c < end) {
+              store_grouped(m, r, c,
+                            finish_grouped((int32_t)((uint32_t)acc[2 * h + e] - (uint32_t)m.zp_w * (uint32_t)xs), (int32_t)row_term, mfp, mexp, m));
+            }
+          }
+        }
+      }
+      __syncthreads();   // `part` may be written again
     }
-    __syncthreads();   // `part` may be written again
-  }
   }
 }
 

@@ -574,48 +574,48 @@ __global__ void __launch_bounds__(kThreads, 2) q4_kernel(const __grid_constant__
   volatile int* abortp = &abort_flag;
   Ring ring = {full, empty, data, &map, 0, 0, 0, 0, 0, true};
   for (;;) {
-  ring.row = (int)(g * a.group_rows + row0);
-  // a long group's passes are shared out along the grid's third axis
-  for (int c0 = begin + (int)blockIdx.z * a.room; c0 < end; c0 += (int)gridDim.z * a.room) {
-    const int n = min(a.room, end - c0);
-    const int tiles = (n * kPieces + 7) / 8;
-    if (kMaxTiles <= 2) {
-      if (tiles == 1) multiply_pass<kType, kPer, 1>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
-      else multiply_pass<kType, kPer, 2>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
-    } else {
-      if (tiles <= 2) multiply_pass<kType, kPer, 2>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
-      else if (tiles <= 4) multiply_pass<kType, kPer, 4>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
-      else multiply_pass<kType, kPer, kMaxTiles>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
-    }
-    if (a.split > 1) cluster_barrier(); else __syncthreads();
-    // every CTA of the cluster finishes its share of the rows
-    const int mine = (kRows + a.split - 1) / a.split;
-    for (int i = threadIdx.x; i < n * mine; i += kThreads) {
-      const int c = i / mine, r = rank * mine + (i - c * mine);
-      if (r >= kRows) continue;
-      float v = 0.f;
-      for (int s = 0; s < a.split; s++) {
-#pragma unroll
-        for (int p = 0; p < kPieces; p++) {
-          const float* at = part + (p * n + c) * kRows + r;
-          v += a.split > 1 ? load_of_rank(at, s) : *at;
-        }
+    ring.row = (int)(g * a.group_rows + row0);
+    // a long group's passes are shared out along the grid's third axis
+    for (int c0 = begin + (int)blockIdx.z * a.room; c0 < end; c0 += (int)gridDim.z * a.room) {
+      const int n = min(a.room, end - c0);
+      const int tiles = (n * kPieces + 7) / 8;
+      if (kMaxTiles <= 2) {
+        if (tiles == 1) multiply_pass<kType, kPer, 1>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
+        else multiply_pass<kType, kPer, 2>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
+      } else {
+        if (tiles <= 2) multiply_pass<kType, kPer, 2>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
+        else if (tiles <= 4) multiply_pass<kType, kPer, 4>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
+        else multiply_pass<kType, kPer, kMaxTiles>(a, ring, xs, part, g, row0, c0, n, slab0, slab1, abortp);
       }
-      if (row0 + r < a.m.rows) store_q4(a.m, g, row0 + r, c0 + c, v * kUnit<kType>);
+      if (a.split > 1) cluster_barrier(); else __syncthreads();
+      // every CTA of the cluster finishes its share of the rows
+      const int mine = (kRows + a.split - 1) / a.split;
+      for (int i = threadIdx.x; i < n * mine; i += kThreads) {
+        const int c = i / mine, r = rank * mine + (i - c * mine);
+        if (r >= kRows) continue;
+        float v = 0.f;
+        for (int s = 0; s < a.split; s++) {
+#pragma unroll
+          for (int p = 0; p < kPieces; p++) {
+            const float* at = part + (p * n + c) * kRows + r;
+            v += a.split > 1 ? load_of_rank(at, s) : *at;
+          }
+        }
+        if (row0 + r < a.m.rows) store_q4(a.m, g, row0 + r, c0 + c, v * kUnit<kType>);
+      }
+      // `part` may be overwritten by the copy engine, or its CTA be gone, once everybody has read it.  Neither needs this pass's
+      // stores to have arrived anywhere, and waiting for them would cost microseconds, so the barrier orders nothing.
+      const bool more = c0 + (int)gridDim.z * a.room < end;
+      if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (a.split > 1) cluster_barrier_relaxed();
+      else if (more) __syncthreads();
+      if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    // `part` may be overwritten by the copy engine, or its CTA be gone, once everybody has read it.  Neither needs this pass's
-    // stores to have arrived anywhere, and waiting for them would cost microseconds, so the barrier orders nothing.
-    const bool more = c0 + (int)gridDim.z * a.room < end;
-    if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    if (a.split > 1) cluster_barrier_relaxed();
-    else if (more) __syncthreads();
-    if (more) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  slot += gridDim.y;
-  if (!nth_group(a.m.groups, a.m.cols, slot, &g, &begin, &end)) break;
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // as between two passes
-  __syncthreads();
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    slot += gridDim.y;
+    if (!nth_group(a.m.groups, a.m.cols, slot, &g, &begin, &end)) break;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // as between two passes
+    __syncthreads();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (abort_flag && threadIdx.x == 0) {
     // give copies in flight a bounded chance to land before the CTA exits: every stage that was filled and not waited for
