@@ -219,7 +219,7 @@ cudaError_t launch_mma(const GroupedI8Mul& m, cudaStream_t stream) {
 // every row then holds them: each lane finds what it needs in its own row of tensor memory, and no pass over the operands
 // and no workspace is needed.  Tiles are narrower then, to leave room in tensor memory.
 //
-// Measured: 8 x 4096 x 4096, 8192 columns 124.7 us (2.2 POP/s; 9 rounds of tiles of 205 columns on average, a stage of 58 KB
+// Measured: 8 x 4096 x 4096, 8192 columns 128 us (2.1 POP/s; 9 rounds of tiles of 205 columns on average, a stage of 58 KB
 // per pair every 375 ns, 11.4 TB/s from L2); 64 x 1024 x 2048, 512 columns 32.6 us (4 us until the first stage is there, then
 // 5.5 TB/s of weights).
 constexpr int kTileM = 128;
@@ -728,8 +728,8 @@ cudaError_t launch_tc(const GroupedI8Mul& m, int sm_count, cudaStream_t stream) 
   const auto column_tiles = [&](int cap) { return max(active, (m.cols + (long long)cap - 1) / cap); };
   const int pairs_m = (m.rows + 2 * kTileM - 1) / (2 * kTileM);
   // Pairs where there is a tile for each: also for few columns, since each CTA then loads half of the tokens (64 experts x
-  // 1024 x 2048, 512 tokens: 32.8 us against 34.8; 8 x 4096 x 4096, 64 tokens: 30.0 against 32.7; 8192 tokens: 138 against
-  // 172).  With fewer tiles than pairs, one CTA per tile uses twice as many SMs (8 x 1024 x 1024, 256 tokens: 10.0 against
+  // 1024 x 2048, 512 tokens: 32.8 us against 34.8; 8 x 4096 x 4096, 64 tokens: 30.0 against 32.7; 8192 tokens, before
+  // later steps: 138 against 172).  With fewer tiles than pairs, one CTA per tile uses twice as many SMs (8 x 1024 x 1024, 256 tokens: 10.0 against
   // 12.3).
   const bool pair = !a.token_sums && m.rows > kTileM && pairs_m * column_tiles(kTcAccCols) >= sm_count / 2;
   a.tiles_m = pair ? pairs_m : (m.rows + kTileM - 1) / kTileM;

@@ -105,8 +105,8 @@ cudaError_t launch_any(const Q4Mul& m, cudaStream_t stream) {
 // are on their way in registers.  The scales of a slab are fetched two slabs ahead, one row per two lanes, and handed to
 // the lanes that need them by shuffles.
 //
-// Measured on one B200: 16384 x 16384, one f16 column 47.6 us (138.5 MB at 2.9 TB/s); 4096 x 16384, 16 bf16 columns 24.9 us;
-// 4096 x 4096, one bf16 column 8.5 us, of which 6 are launch, set-up and the cluster's barriers.  The large one is bound by
+// Measured on one B200: 16384 x 16384, one f16 column 48.4 us (138.5 MB at 2.9 TB/s); 4096 x 16384, 16 bf16 columns 25.3 us;
+// 4096 x 4096, one bf16 column 8.6 us, of which 6 are launch, set-up and the cluster's barriers.  The large one is bound by
 // instruction issue and the ALU pipe (45 instructions per 16 rows x 32 deep, 25 of them the arithmetic above): the same
 // kernel without its arithmetic takes 28 us.
 //
@@ -685,7 +685,7 @@ cudaError_t launch_tensor(const Q4Mul& m, int sm_count, cudaStream_t stream) {
   // Columns per pass, a whole number of MMA tiles: 16 half or 5 fp32 ones (two tiles), or 32 and 16 (four and six), whose
   // warps hold more sums and so hide less of each other's latency.  A group of about 12 columns or fewer is better served
   // by several narrow passes side by side (16 groups x 2048 x 2048, 131 columns: bf16 26 us against 36, fp32 45 against 50),
-  // one of 32 by wide passes (8 x 1024 x 1024, 256 fp32 columns: 34 us against 50).
+  // one of 32 by wide passes (8 x 1024 x 1024, 256 fp32 columns: 27 us against 50).
   const long long share = m.groups.offsets ? (m.cols + (long long)m.groups.count - 1) / m.groups.count : m.cols;
   const bool few = m.groups.offsets ? share <= 12 : share * pieces <= 16;
   a.room = few ? 16 / pieces : (pieces == 3 ? 16 : 32);
